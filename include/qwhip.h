@@ -536,6 +536,83 @@ qwhip_status qwhip_repack_mlx_affine_switch_gate_up(qwhip_stream_t s, const void
                                                     uint32_t inter, uint32_t cols, uint32_t bits, uint32_t group,
                                                     void* dst_blocks, uint32_t* refused);
 
+/* ---- MXFP4: microscaled 4-bit floating point ------------------------------------ */
+/* 32 elements of e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives) under one power-of-two scale byte e8m0 (2^(byte - 127),
+ * 255 = NaN), as 4-bit float checkpoints store them, in two planes.  The reference has no such container: the doors stand
+ * beside the integer containers' (quantiser, dequant, decode GEMV, prefill GEMM), in the standard basis.
+ * Every door checks its arguments before it enqueues, allocates nothing, keeps no state between calls and only launches
+ * kernels (a call can be captured); rows beyond the ones that a call names are not written.  No door uses the stream's scratch. */
+typedef struct qwhip_mxfp4_view {
+    const void* codes;     /* device, 16-byte aligned: row r at byte r * ld / 2, element 2 i in the low half of byte i */
+    const void* scales;    /* device: row r at byte r * ld / 32, one byte for 32 elements */
+    uint64_t codes_bytes;  /* what the caller's regions hold from these pointers on */
+    uint64_t scales_bytes;
+    uint32_t n;            /* rows */
+    uint32_t k;            /* columns, a multiple of 32 */
+    uint32_t ld;           /* elements from row to row, a multiple of 32 (0 = k) */
+} qwhip_mxfp4_view;
+/* QWHIP_OK, QWHIP_E_BAD_WEIGHTS (rows, columns, pitch, plane sizes, alignment) or QWHIP_E_NULL. */
+qwhip_status qwhip_mxfp4_view_validate(const qwhip_mxfp4_view* v);
+/* Weights at load time, or activations in front of qwhip_mxfp4_gemm: src [rows, ld] f32, f16 or bf16 (ld in elements, 0 = k;
+ * rows 16-byte aligned, k % 32 == 0) -> codes [rows, k / 2], scales [rows, k / 32], both tight.  A block's scale is
+ * 2^(floor(log2 max|v|) - 2), at least 2^-127; an element is the nearest e2m1 value of v / scale, ties to the even code,
+ * magnitudes over 6 to 6, the sign kept.  A block with an infinity or a NaN gets scale byte 255 and codes 0 (it reads as NaN).
+ * values (may be NULL; 16-byte aligned): what the codes stand for, [rows, k] tight in src's type, exact; codes and values 16-byte
+ * aligned.  src, codes, scales and values do not overlap. */
+qwhip_status qwhip_quantize_mxfp4(qwhip_stream_t s, const void* src, uint32_t src_dtype, uint32_t rows, uint32_t k, uint32_t ld,
+                                  void* codes, void* scales, void* values);
+/* out [n, k] row-major, tight, 16-byte aligned: the values of a bank; exact in f32 and bf16 (from 2^128 on,
+ * which scale bytes 253 and 254 reach, infinity), rounded where f16 does not hold them. */
+qwhip_status qwhip_dequant_mxfp4(qwhip_stream_t s, const qwhip_mxfp4_view* v, void* out, uint32_t out_dtype);
+/* y [m, n] = X . W^T of two quantised operands, w [n, k] and x [m = x->n, k], any m (0 rows: nothing to do), n and k % 32 == 0; y f32,
+ * f16 or bf16 with row pitch ldy elements (0 = n).  fp32 accumulation of exact products, one rounding at the store.
+ * workspace (may be NULL; 16-byte aligned) lets few tiles split k over more compute units: fp32 planes of m * n elements, at
+ * most qwhip_mxfp4_gemm_workspace_bytes(m, n, k) bytes of it.  The planes are summed in a fixed order; which form runs
+ * follows from m, n, k, the pitches and the room in the workspace, never from its contents.  Two calls that overlap in time
+ * take two workspaces. */
+qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const qwhip_mxfp4_view* x, void* y, uint32_t y_dtype,
+                              uint32_t ldy, void* workspace, uint64_t workspace_bytes);
+uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
+/* Decode / verify: y [m, n] = x . W^T for m = 1..16 rows (0: nothing to do) of f16 or bf16 activations [m, k], tight and 16-byte
+ * aligned, not quantised; y16 (f16) and / or y32 (f32), at least one.  Every weight byte is read once for all rows; fp32 accumulation. */
+qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_view* w, const void* x, uint32_t x_dtype, uint32_t m, void* y16,
+                              float* y32);
+
+/* ---- from logits to the token ------------------------------------------------------ */
+/* What a step of a batch applies to its logits before a token is chosen, in this order, in fp32:
+ *   seen in the row's history (prompt or answer): l = l > 0 ? l / repetition : l * repetition
+ *   c > 0 times in its answer:                    l = l - frequency * c - presence
+ *   listed with a bias:                           l = l + value (of two entries for a token the later one holds)
+ *   not allowed by its mask:                      l = -inf
+ * All pointers are device memory.  A part whose pointer is NULL is left out. */
+typedef struct qwhip_logits_rules {
+    const int32_t* history;     /* [rows, ld_history] tokens, prompt then answer; a token outside 0 .. n - 1 is skipped */
+    const int32_t* prompt_len;  /* [rows]: the first prompt_len tokens are the prompt (NULL: all are answer) */
+    const int32_t* total_len;   /* [rows]: tokens of the row's history (clamped to 0 .. ld_history); required with history */
+    const float* repetition;    /* [rows], > 0 (NULL: 1) */
+    const float* presence;      /* [rows] (NULL: 0) */
+    const float* frequency;     /* [rows] (NULL: 0) */
+    const int32_t* bias_off;    /* [rows + 1]: row r has the entries bias_off[r] .. bias_off[r + 1] - 1 (clamped to bias_count) */
+    const int32_t* bias_tok;    /* [bias_count] */
+    const float* bias_val;      /* [bias_count] */
+    const uint32_t* allowed;    /* [allowed_rows, ld_allowed] words: token t is allowed where bit t % 32 of word t / 32 is set */
+    const int32_t* allowed_row; /* [rows]: the row's mask, anything outside 0 .. allowed_rows - 1: none (NULL: row r has mask r) */
+    uint32_t ld_history;
+    uint32_t bias_count;
+    uint32_t allowed_rows;
+    uint32_t ld_allowed;        /* words from mask to mask, at least ceil(n / 32) */
+} qwhip_logits_rules;
+/* logits [rows, n] f32, f16 or bf16 with row pitch ld (0 = n) -> out (same type, row pitch ld_out; may be logits itself at the
+ * same pitch; NULL: not written) and tokens i32 [rows] (NULL: not asked for): the largest of the row's fp32 results, before they
+ * are rounded to out's type, by the key rule of qwhip_argmax_f32 (NaN never wins against a number, ties to the lower token); -1
+ * where nothing is above -inf, as behind a mask that allows no token.  Tokens need a workspace (8-byte aligned) of
+ * qwhip_logits_workspace_bytes(rows, n) bytes, which the call writes before it reads; two calls that overlap in time take two.
+ * rows <= 65535 (0: nothing to do), n < 2^30. */
+qwhip_status qwhip_logits_process(qwhip_stream_t s, const qwhip_logits_rules* rules, const void* logits, uint32_t dtype,
+                                  uint32_t rows, uint32_t n, uint32_t ld, void* out, uint32_t ld_out, int32_t* tokens,
+                                  void* workspace, uint64_t workspace_bytes);
+uint64_t qwhip_logits_workspace_bytes(uint32_t rows, uint32_t n);
+
 #ifdef __cplusplus
 }
 #endif

@@ -39,6 +39,17 @@ class Caps(C.Structure):
                 ("hbm_bytes", C.c_uint64), ("clock_khz", C.c_uint32), ("has_mfma_f16", C.c_uint32)]
 
 
+class Mxfp4View(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("codes_bytes", C.c_uint64), ("scales_bytes", C.c_uint64),
+                ("n", C.c_uint32), ("k", C.c_uint32), ("ld", C.c_uint32)]
+
+
+class LogitsRules(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("history", "prompt_len", "total_len", "repetition", "presence", "frequency", "bias_off", "bias_tok",
+                                                "bias_val", "allowed", "allowed_row")]
+    _fields_ += [(name, C.c_uint32) for name in ("ld_history", "bias_count", "allowed_rows", "ld_allowed")]
+
+
 _P = C.c_void_p
 _U32 = C.c_uint32
 _U64 = C.c_uint64
@@ -117,6 +128,14 @@ SIGNATURES = {
     "qwhip_gemv_f32": (C.c_int32, [_P, _WV, _P, _U32, _U32, C.c_float, _P]),
     "qwhip_h32_f32": (C.c_int32, [_P, _P, _P, _U32, _U32]),
     "qwhip_rmsnorm": (C.c_int32, [_P, _P, _P, _P, _U32, _U32, C.c_float, _U32, _P]),
+    "qwhip_mxfp4_view_validate": (C.c_int32, [C.POINTER(Mxfp4View)]),
+    "qwhip_quantize_mxfp4": (C.c_int32, [_P, _P, _U32, _U32, _U32, _U32, _P, _P, _P]),
+    "qwhip_dequant_mxfp4": (C.c_int32, [_P, C.POINTER(Mxfp4View), _P, _U32]),
+    "qwhip_mxfp4_gemm": (C.c_int32, [_P, C.POINTER(Mxfp4View), C.POINTER(Mxfp4View), _P, _U32, _U32, _P, _U64]),
+    "qwhip_mxfp4_gemm_workspace_bytes": (_U64, [_U32, _U32, _U32]),
+    "qwhip_mxfp4_gemv": (C.c_int32, [_P, C.POINTER(Mxfp4View), _P, _U32, _U32, _P, _P]),
+    "qwhip_logits_process": (C.c_int32, [_P, C.POINTER(LogitsRules), _P, _U32, _U32, _U32, _U32, _P, _U32, _P, _P, _U64]),
+    "qwhip_logits_workspace_bytes": (_U64, [_U32, _U32]),
     "qwhip_repack_mlx_affine": (C.c_int32, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
     "qwhip_repack_mlx_affine_switch_gate_up": (C.c_int32, [_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P]),
 }
