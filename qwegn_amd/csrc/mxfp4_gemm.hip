@@ -64,8 +64,7 @@ __global__ __launch_bounds__(256) void qw_mx_gemm_plain_kernel(qw_mx_operand w, 
 }
 
 // ------------------------------------------------------------------------------------------------
-// The tiled kernel.  A workgroup of four waves (2 x 2) owns a tile of 32 MF rows of X by 32 NF rows of W, a wave 16 MF x 16 NF of it, all
-// sums in registers.  Both operands pass through LDS in stages of 256 columns: a row's 128 bytes as eight pieces of 16 (one block each),
+// The tiled kernel.  A workgroup of WM x WN waves owns a tile of X's rows by W's rows, a wave 16 MF x 16 NF of it, all sums in registers.  Both operands pass through LDS in stages of 256 columns: a row's 128 bytes as eight pieces of 16 (one block each),
 // piece c of row r at place c ^ ((r >> 1) & 7), so that the 16 rows that a fragment read touches lie on all banks.  Scales come in steps of
 // two stages, 16 bytes of a row: the scales of four fragments' rows in one block column form one word (the matrix instruction picks the
 // byte), transposed inside lane quads on their way into LDS.
@@ -80,10 +79,11 @@ __device__ __forceinline__ void qw_static_for(F&& f) {
 
 // c += a . b under bytes OA and OB of the scale words.  Written out so that the sums stay in one set of accumulation registers: a tile's 256
 // of them and what else is alive fill the file, and left to itself the compiler moved sums about (250 moves beside 128 of these in the loop).
-// Operands come from LDS reads, for which the compiler waits; sums are written by nothing but these and read behind QW_MX_DRAIN.
+// Operands come from LDS reads, for which the compiler waits, or from vector instructions, which need the two wait states in front (they
+// pass while the unit is busy with the instruction before); sums are written by nothing but these and read behind QW_MX_DRAIN.
 template <int OA, int OB>
 __device__ __forceinline__ void qw_mx_mfma_at(u4_t a, uint32_t sa, u4_t b, uint32_t sb, f4_t& c) {
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
                  : "+a"(c)
                  : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(OA & 1), "n"(OB & 1), "n"(OA >> 1), "n"(OB >> 1));
 }
@@ -95,23 +95,25 @@ struct qw_mx_tile_args {
     uint32_t blocks, ldy, tiles_m, tiles_n;
 };
 
-template <int MF, int NF>
+template <int MF, int NF, int WM, int WN>
 struct qw_mx_tile {
-    static constexpr uint32_t BM = 32u * MF, BN = 32u * NF, ROWS = BM + BN;
-    static constexpr uint32_t GX = (MF + 3) / 4, GW = (NF + 3) / 4, GROUPS = 2u * (GX + GW);   // groups of four fragments, a wave's own
+    static constexpr uint32_t WAVES = WM * WN, THREADS = 64u * WAVES, BM = 16u * MF * WM, BN = 16u * NF * WN, ROWS = BM + BN;
+    static constexpr uint32_t GX = (MF + 3) / 4, GW = (NF + 3) / 4, GROUPS = WM * GX + WN * GW;   // groups of four fragments, a wave's own
     static constexpr uint32_t CODES = ROWS * 128u;                    // a stage's codes; two of them, then two steps' scales
     static constexpr uint32_t SCALES = GROUPS * 1024u;
-    static constexpr uint32_t PIECES = MF + NF;                       // 16-byte pieces of a stage that a thread carries
-    static constexpr uint32_t SROWS = (GROUPS + 3u) / 4u;             // rows whose scales of a step a thread carries
+    static constexpr uint32_t STEP = THREADS / 8u;                    // a thread carries 16-byte pieces of rows STEP apart
+    static constexpr uint32_t XPIECES = BM / STEP, PIECES = ROWS / STEP;
+    static constexpr uint32_t SROWS = (GROUPS + WAVES - 1u) / WAVES;  // rows whose scales of a step a thread carries
+    static_assert(BM % STEP == 0 && BN % STEP == 0, "whole pieces");
     static constexpr uint32_t LDS = 2u * (CODES + SCALES);
 };
 
-template <int MF, int NF, int DT>
-__global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_tile_args a) {
-    using T = qw_mx_tile<MF, NF>;
+template <int MF, int NF, int WM, int WN, int DT>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_kernel(const qw_mx_tile_args a) {
+    using T = qw_mx_tile<MF, NF, WM, WN>;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), i = lane & 15u, g = lane >> 4;
-    const uint32_t wm = wave & 1u, wn = wave >> 1;
+    const uint32_t wm = wave % WM, wn = wave / WM;
 
     // workgroups are dealt to the eight XCDs in turn: an XCD takes a contiguous run of labels, and labels walk bands four tiles tall
     const uint32_t total = a.tiles_m * a.tiles_n, per_xcd = (total + 7u) / 8u, label = (blockIdx.x & 7u) * per_xcd + (blockIdx.x >> 3);
@@ -120,20 +122,20 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     // the last tile of a side ends with the operand: the rows that it shares with its neighbour get the same bits from both
     const uint32_t n0 = min((in_band / tall) * T::BN, a.w.rows - T::BN), m0 = min((4u * band + in_band % tall) * T::BM, a.x.rows - T::BM);
 
-    // what a thread carries of a stage: piece c = tid & 7 of rows tid / 8 + 32 j, X's rows first
+    // what a thread carries of a stage: piece c = tid & 7 of rows tid / 8 + STEP j, X's rows first
     const uint32_t c = tid & 7u, row0 = tid >> 3;
     const uint32_t xpitch = a.x.ld32 * 16u, wpitch = a.w.ld32 * 16u, xrow = row0 * xpitch, wrow = row0 * wpitch;
     const uint8_t* const xc = a.x.codes + (uint64_t)m0 * xpitch;
     const uint8_t* const wc = a.w.codes + (uint64_t)n0 * wpitch;
-    const uint32_t park = row0 * 128u + ((c ^ ((row0 >> 1) & 7u)) << 4);   // + 4096 j: 32 rows on, the same place in the row
+    const uint32_t park = row0 * 128u + ((c ^ ((row0 >> 1) & 7u)) << 4);   // STEP rows on, the same place in the row
     // the scales that it carries: of row i of fragment f of a group, lanes 4 i + f; a step's 16 bytes
     const uint8_t* sbase[T::SROWS];
     uint32_t srow[T::SROWS], sgroup[T::SROWS];
 #pragma unroll
     for (uint32_t t = 0; t < T::SROWS; ++t) {
-        const uint32_t grp = min(4u * t + wave, T::GROUPS - 1u);
-        const bool of_x = grp < 2u * T::GX;
-        const uint32_t gg = of_x ? grp : grp - 2u * T::GX, per = of_x ? T::GX : T::GW, span = of_x ? 16u * MF : 16u * NF;
+        const uint32_t grp = min(T::WAVES * t + wave, T::GROUPS - 1u);
+        const bool of_x = grp < WM * T::GX;
+        const uint32_t gg = of_x ? grp : grp - WM * T::GX, per = of_x ? T::GX : T::GW, span = of_x ? 16u * MF : 16u * NF;
         const uint32_t at = min((gg / per) * span + (gg % per) * 64u + 16u * (lane & 3u) + (lane >> 2), (of_x ? T::BM : T::BN) - 1u);
         sgroup[t] = grp;
         sbase[t] = of_x ? a.x.scales + (uint64_t)m0 * a.x.ld32 : a.w.scales + (uint64_t)n0 * a.w.ld32;
@@ -145,8 +147,8 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     auto fetch_codes = [&](uint32_t st, auto j) {
         const uint32_t off = min(st * 8u + c, a.blocks - 1u) * 16u;   // behind the last block: any block, under scales of zero
         constexpr uint32_t J = decltype(j)::value;
-        if constexpr (J < MF) staged[J] = *(const u4_t*)(xc + (uint64_t)(32u * J) * xpitch + (xrow + off));
-        else staged[J] = *(const u4_t*)(wc + (uint64_t)(32u * (J - MF)) * wpitch + (wrow + off));
+        if constexpr (J < T::XPIECES) staged[J] = *(const u4_t*)(xc + (uint64_t)(T::STEP * J) * xpitch + (xrow + off));
+        else staged[J] = *(const u4_t*)(wc + (uint64_t)(T::STEP * (J - T::XPIECES)) * wpitch + (wrow + off));
     };
     auto fetch_scales = [&](uint32_t step) {
         const uint32_t b = step * 16u;
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     };
     auto park_codes = [&](uint32_t st, auto j) {
         constexpr uint32_t J = decltype(j)::value;
-        *(u4_t*)(lds + (st & 1u) * T::CODES + park + 4096u * J) = staged[J];
+        *(u4_t*)(lds + (st & 1u) * T::CODES + park + T::STEP * 128u * J) = staged[J];
     };
     // word q of lane 4 i + f has the scales of half stage q of row (f, i), a byte for each block column: after the transpose inside the quad
     // it has the scales of block column f, a byte for each fragment
@@ -175,38 +177,34 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     auto park_scales = [&](uint32_t step) {
 #pragma unroll
         for (uint32_t t = 0; t < T::SROWS; ++t) {
-            u4_t o;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (uint32_t q = 0; q < 4; ++q) {   // to [group][half stage][row][block column]
                 const uint32_t v = sstaged[t][q], p = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
                 const uint32_t u = __builtin_amdgcn_perm(p, v, pick1), r = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x4E, 0xF, 0xF, true);
-                o[q] = __builtin_amdgcn_perm(r, u, pick2);
+                *(uint32_t*)(lds + 2u * T::CODES + (step & 1u) * T::SCALES + sgroup[t] * 1024u + q * 256u + lane * 4u) = __builtin_amdgcn_perm(r, u, pick2);
             }
-            *(u4_t*)(lds + 2u * T::CODES + (step & 1u) * T::SCALES + sgroup[t] * 1024u + lane * 16u) = o;   // [group][row][block column][half stage]
         }
     };
-    // a wave's fragments of half a stage, and its scales of a step
-    struct frags {
-        u4_t x[MF], w[NF];
-    };
-    struct words {
-        u4_t x[T::GX], w[T::GW];
-    };
+    // a wave's fragments and scales of half a stage: W's fragments are each read again when their matrix instructions are out, the rest twice
+    u4_t x[2][MF], w[NF];
+    uint32_t sx[2][T::GX], sw[2][T::GW];
     const uint32_t key = (i >> 1) & 7u;   // (row >> 1) & 7 of every fragment's row i: rows of fragments are 16 apart
     const uint32_t xat = (wm * 16u * MF + i) * 128u, wat = (T::BM + wn * 16u * NF + i) * 128u;
     const uint32_t place[2] = {((g ^ key) << 4), (((4u + g) ^ key) << 4)};
-    auto read_x = [&](frags& f, uint32_t st, uint32_t h, auto j) {
-        f.x[decltype(j)::value] = *(const u4_t*)(lds + (st & 1u) * T::CODES + xat + place[h] + 2048u * decltype(j)::value);
+    auto read_x = [&](uint32_t st, auto h, auto j) {
+        x[decltype(h)::value][decltype(j)::value] = *(const u4_t*)(lds + (st & 1u) * T::CODES + xat + place[decltype(h)::value] + 2048u * decltype(j)::value);
     };
-    auto read_w = [&](frags& f, uint32_t st, uint32_t h, auto j) {
-        f.w[decltype(j)::value] = *(const u4_t*)(lds + (st & 1u) * T::CODES + wat + place[h] + 2048u * decltype(j)::value);
+    auto read_w = [&](uint32_t st, auto h, auto j) {
+        w[decltype(j)::value] = *(const u4_t*)(lds + (st & 1u) * T::CODES + wat + place[decltype(h)::value] + 2048u * decltype(j)::value);
     };
-    auto read_scales = [&](words& s, uint32_t step) {
-        const uint32_t at = 2u * T::CODES + (step & 1u) * T::SCALES + (4u * i + g) * 16u;
+    const uint32_t sat = 2u * T::CODES + (4u * i + g) * 4u;
+    auto read_scales = [&](uint32_t st, auto h) {
+        constexpr int H = decltype(h)::value;
+        const uint32_t at = sat + ((st >> 1) & 1u) * T::SCALES + (2u * (st & 1u) + H) * 256u;
 #pragma unroll
-        for (uint32_t q = 0; q < T::GX; ++q) s.x[q] = *(const u4_t*)(lds + at + (wm * T::GX + q) * 1024u);
+        for (uint32_t q = 0; q < T::GX; ++q) sx[H][q] = *(const uint32_t*)(lds + at + (wm * T::GX + q) * 1024u);
 #pragma unroll
-        for (uint32_t q = 0; q < T::GW; ++q) s.w[q] = *(const u4_t*)(lds + at + (2u * T::GX + wn * T::GW + q) * 1024u);
+        for (uint32_t q = 0; q < T::GW; ++q) sw[H][q] = *(const uint32_t*)(lds + at + (WM * T::GX + wn * T::GW + q) * 1024u);
     };
     f4_t acc[NF][MF];
 #pragma unroll
@@ -217,12 +215,11 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
             asm volatile("" : "+a"(acc[n][m]));   // in place before the wait below
         }
     QW_MX_DRAIN();
-    auto multiply = [&](const frags& f, const words& s, auto q, auto n) {
-        constexpr int N = decltype(n)::value, Q = decltype(q)::value;
+    auto multiply = [&](auto h, auto n) {
+        constexpr int N = decltype(n)::value, H = decltype(h)::value;
         qw_static_for<MF>([&](auto m) {
             constexpr int M = decltype(m)::value;
-            const uint32_t sw = s.w[N >> 2][Q], sx = s.x[M >> 2][Q];
-            qw_mx_mfma_at<N & 3, M & 3>(f.w[N], sw, f.x[M], sx, acc[N][M]);
+            qw_mx_mfma_at<N & 3, M & 3>(w[N], sw[H][N >> 2], x[H][M], sx[H][M >> 2], acc[N][M]);
         });
     };
 
@@ -232,45 +229,51 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     park_scales(0);
     qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(1u, stages - 1u), j); });
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    frags f0, f1;
-    words s0, s1;
-    read_scales(s0, 0);
-    qw_static_for<MF>([&](auto j) { read_x(f0, 0, 0, j); });
-    qw_static_for<NF>([&](auto j) { read_w(f0, 0, 0, j); });
-    constexpr int PER = (int)(T::PIECES + NF - 1) / NF;   // memory instructions of a kind beside the MF matrix instructions of one fragment of W
+    constexpr std::integral_constant<int, 0> H0{};
+    constexpr std::integral_constant<int, 1> H1{};
+    read_scales(0, H0);
+    qw_static_for<MF>([&](auto j) { read_x(0, H0, j); });
+    qw_static_for<NF>([&](auto j) { read_w(0, H0, j); });
     // A stage.  First half: its matrix instructions, the second half's fragments on their way in, the next stage into the other buffer.
     // Second half: the stage after the next one is asked for, the next one's first fragments are on their way in.  Behind the last stage
     // the last one again, into a buffer that nobody reads.
+    constexpr int PER = (int)(T::PIECES + NF - 1) / NF, PERX = (MF + NF - 1) / NF;   // beside the MF matrix instructions of a fragment of W
     auto stage = [&](uint32_t st, auto parity) {
         constexpr int P = decltype(parity)::value;
         const uint32_t after = min(st + 2u, stages - 1u), step = st >> 1;
+        read_scales(st, H1);
         if constexpr (P == 0) fetch_scales(min(step + 1u, (stages - 1u) >> 1));
         qw_static_for<NF>([&](auto n) {
             constexpr int N = decltype(n)::value;
+            qw_static_for<PERX>([&](auto k) {
+                constexpr int J = N * PERX + decltype(k)::value;
+                if constexpr (J < MF) read_x(st, H1, std::integral_constant<int, J>{});
+            });
             qw_static_for<PER>([&](auto k) {
                 constexpr int J = N * PER + decltype(k)::value;
-                if constexpr (J < MF) read_x(f1, st, 1, std::integral_constant<int, J>{});
-                else if constexpr (J < MF + NF) read_w(f1, st, 1, std::integral_constant<int, J - MF>{});
                 if constexpr (J < (int)T::PIECES) park_codes(st + 1u, std::integral_constant<int, J>{});
             });
             if constexpr (P == 1 && N == NF / 2) park_scales(step + 1u);
-            multiply(f0, s0, std::integral_constant<int, 2 * P>{}, n);
+            multiply(H0, n);
+            read_w(st, H1, n);
             __builtin_amdgcn_sched_barrier(0);
         });
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if constexpr (P == 1) read_scales(s1, step + 1u);
+        read_scales(st + 1u, H0);
         qw_static_for<NF>([&](auto n) {
             constexpr int N = decltype(n)::value;
+            qw_static_for<PERX>([&](auto k) {
+                constexpr int J = N * PERX + decltype(k)::value;
+                if constexpr (J < MF) read_x(st + 1u, H0, std::integral_constant<int, J>{});
+            });
             qw_static_for<PER>([&](auto k) {
                 constexpr int J = N * PER + decltype(k)::value;
-                if constexpr (J < MF) read_x(f0, st + 1u, 0, std::integral_constant<int, J>{});
-                else if constexpr (J < MF + NF) read_w(f0, st + 1u, 0, std::integral_constant<int, J - MF>{});
                 if constexpr (J < (int)T::PIECES) fetch_codes(after, std::integral_constant<int, J>{});
             });
-            multiply(f1, s0, std::integral_constant<int, 2 * P + 1>{}, n);
+            multiply(H1, n);
+            read_w(st + 1u, H0, n);
             __builtin_amdgcn_sched_barrier(0);
         });
-        if constexpr (P == 1) s0 = s1;
     };
     for (uint32_t st = 0; st < stages; st += 2u) {
         stage(st, std::integral_constant<int, 0>{});
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     using E = std::conditional_t<DT == QWHIP_F32, float, std::conditional_t<DT == QWHIP_F16, h1_t, __bf16>>;
     typedef E e4_t __attribute__((ext_vector_type(4)));
     constexpr uint32_t PITCH = 16u * NF * sizeof(E) + 16u, ROW16 = NF * sizeof(E);   // bytes of a row in LDS; its 16-byte pieces
-    static_assert(4u * 16u * PITCH <= T::LDS, "the waves' rows fit the stages' place");
+    static_assert(T::WAVES * 16u * PITCH <= T::LDS, "the waves' rows fit the stages' place");
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* const own = lds + wave * 16u * PITCH;
     const bool pieces = (((uint64_t)a.ldy | n0) * sizeof(E) & 15u) == 0u && ((uintptr_t)a.y & 15u) == 0u;
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
 #pragma unroll
             for (uint32_t k = 0; k < 16u * ROW16 / 64u; ++k) {
                 const uint32_t id = 64u * k + lane, r = id / ROW16, p = id % ROW16;
-                *(u4_t*)((uint8_t*)(y + (uint64_t)r * a.ldy) + 16u * p) = *(const u4_t*)(own + r * PITCH + 16u * p);
+                __builtin_nontemporal_store(*(const u4_t*)(own + r * PITCH + 16u * p), (u4_t*)((uint8_t*)(y + (uint64_t)r * a.ldy) + 16u * p));
             }
         } else {
 #pragma unroll 1
@@ -314,14 +317,14 @@ __global__ __launch_bounds__(256, 1) void qw_mx_gemm_tile_kernel(const qw_mx_til
     }
 }
 
-template <int MF, int NF>
+template <int MF, int NF, int WM, int WN>
 static void qw_mx_launch_tile(qwhip_stream_t s, qw_mx_tile_args a, uint32_t y_dtype) {
-    using T = qw_mx_tile<MF, NF>;
+    using T = qw_mx_tile<MF, NF, WM, WN>;
     a.tiles_m = qwhip_cdiv(a.x.rows, T::BM), a.tiles_n = qwhip_cdiv(a.w.rows, T::BN);
-    const dim3 grid(8u * qwhip_cdiv(a.tiles_m * a.tiles_n, 8u)), block(256);
-    if (y_dtype == QWHIP_F32) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, QWHIP_F32>), grid, block, 0, s->stream, a);
-    else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, QWHIP_F16>), grid, block, 0, s->stream, a);
-    else hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, QWHIP_BF16>), grid, block, 0, s->stream, a);
+    const dim3 grid(8u * qwhip_cdiv(a.tiles_m * a.tiles_n, 8u)), block(T::THREADS);
+    if (y_dtype == QWHIP_F32) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_F32>), grid, block, 0, s->stream, a);
+    else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_F16>), grid, block, 0, s->stream, a);
+    else hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_BF16>), grid, block, 0, s->stream, a);
 }
 
 extern "C" uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
@@ -352,7 +355,7 @@ extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_vie
     const qw_mx_operand ow = {(const uint8_t*)w->codes, (const uint8_t*)w->scales, w->n, qw_mxfp4_ld(w) / 32u};
     const qw_mx_operand ox = {(const uint8_t*)x->codes, (const uint8_t*)x->scales, x->n, qw_mxfp4_ld(x) / 32u};
     if (x->n >= 256u && w->n >= 256u && w->k >= 128u && ow.ld32 < (1u << 18) && ox.ld32 < (1u << 18)) {   // 32-bit offsets inside a tile
-        qw_mx_launch_tile<8, 8>(s, {ow, ox, y, w->k / 32u, ldy, 0, 0}, y_dtype);
+        qw_mx_launch_tile<4, 8, 4, 2>(s, {ow, ox, y, w->k / 32u, ldy, 0, 0}, y_dtype);
         QWHIP_TRY_HIP(hipGetLastError());
         return QWHIP_OK;
     }
