@@ -123,11 +123,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     const uint32_t n0 = min((in_band / tall) * T::BN, a.w.rows - T::BN), m0 = min((4u * band + in_band % tall) * T::BM, a.x.rows - T::BM);
 
     // what a thread carries of a stage: piece c = tid & 7 of rows tid / 8 + STEP j, X's rows first
-    const uint32_t c = tid & 7u, row0 = tid >> 3;
+    const uint32_t row0 = tid >> 3, c = (tid & 7u) ^ ((row0 >> 1) & 7u);
     const uint32_t xpitch = a.x.ld32 * 16u, wpitch = a.w.ld32 * 16u, xrow = row0 * xpitch, wrow = row0 * wpitch;
     const uint8_t* const xc = a.x.codes + (uint64_t)m0 * xpitch;
     const uint8_t* const wc = a.w.codes + (uint64_t)n0 * wpitch;
-    const uint32_t park = row0 * 128u + ((c ^ ((row0 >> 1) & 7u)) << 4);   // STEP rows on, the same place in the row
     // the scales that it carries: of row i of fragment f of a group, lanes 4 i + f; a step's 16 bytes
     const uint8_t* sbase[T::SROWS];
     uint32_t srow[T::SROWS], sgroup[T::SROWS];
@@ -142,13 +141,15 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
         srow[t] = at * (of_x ? a.x.ld32 : a.w.ld32);
     }
 
-    u4_t staged[T::PIECES], sstaged[T::SROWS];
+    u4_t sstaged[T::SROWS];
     const uint32_t stages = (a.blocks + 7u) / 8u;
-    auto fetch_codes = [&](uint32_t st, auto j) {
+    // 1 KB of a stage from memory into LDS, eight rows of a wave: lane l's 16 bytes land at place l & 7 of row l >> 3
+    auto fetch_codes = [&](uint32_t st, uint32_t into, auto j) {
         const uint32_t off = min(st * 8u + c, a.blocks - 1u) * 16u;   // behind the last block: any block, under scales of zero
         constexpr uint32_t J = decltype(j)::value;
-        if constexpr (J < T::XPIECES) staged[J] = *(const u4_t*)(xc + (uint64_t)(T::STEP * J) * xpitch + (xrow + off));
-        else staged[J] = *(const u4_t*)(wc + (uint64_t)(T::STEP * (J - T::XPIECES)) * wpitch + (wrow + off));
+        const uint8_t* const from = J < T::XPIECES ? xc + (uint64_t)(T::STEP * J) * xpitch + (xrow + off) : wc + (uint64_t)(T::STEP * (J - T::XPIECES)) * wpitch + (wrow + off);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                         (__attribute__((address_space(3))) void*)(lds + (into & 1u) * T::CODES + (T::STEP * J + 8u * wave) * 128u), 16, 0, 0);
     };
     auto fetch_scales = [&](uint32_t step) {
         const uint32_t b = step * 16u;
@@ -166,10 +167,6 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
                     sstaged[t][q] = cut < 32u ? v >> cut : 0u;
                 }
         }
-    };
-    auto park_codes = [&](uint32_t st, auto j) {
-        constexpr uint32_t J = decltype(j)::value;
-        *(u4_t*)(lds + (st & 1u) * T::CODES + park + T::STEP * 128u * J) = staged[J];
     };
     // word q of lane 4 i + f has the scales of half stage q of row (f, i), a byte for each block column: after the transpose inside the quad
     // it has the scales of block column f, a byte for each fragment
@@ -223,12 +220,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
         });
     };
 
-    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(0, j); });
     fetch_scales(0);
-    qw_static_for<T::PIECES>([&](auto j) { park_codes(0, j); });
+    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(0, 0, j); });
     park_scales(0);
-    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(1u, stages - 1u), j); });
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(1u, stages - 1u), 1, j); });
     constexpr std::integral_constant<int, 0> H0{};
     constexpr std::integral_constant<int, 1> H1{};
     read_scales(0, H0);
@@ -249,16 +245,12 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
                 constexpr int J = N * PERX + decltype(k)::value;
                 if constexpr (J < MF) read_x(st, H1, std::integral_constant<int, J>{});
             });
-            qw_static_for<PER>([&](auto k) {
-                constexpr int J = N * PER + decltype(k)::value;
-                if constexpr (J < (int)T::PIECES) park_codes(st + 1u, std::integral_constant<int, J>{});
-            });
             if constexpr (P == 1 && N == NF / 2) park_scales(step + 1u);
             multiply(H0, n);
             read_w(st, H1, n);
             __builtin_amdgcn_sched_barrier(0);
         });
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         read_scales(st + 1u, H0);
         qw_static_for<NF>([&](auto n) {
             constexpr int N = decltype(n)::value;
@@ -268,7 +260,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
             });
             qw_static_for<PER>([&](auto k) {
                 constexpr int J = N * PER + decltype(k)::value;
-                if constexpr (J < (int)T::PIECES) fetch_codes(after, std::integral_constant<int, J>{});
+                if constexpr (J < (int)T::PIECES) fetch_codes(after, st, std::integral_constant<int, J>{});
             });
             multiply(H1, n);
             read_w(st + 1u, H0, n);
@@ -290,7 +282,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     typedef E e4_t __attribute__((ext_vector_type(4)));
     constexpr uint32_t PITCH = 16u * NF * sizeof(E) + 16u, ROW16 = NF * sizeof(E);   // bytes of a row in LDS; its 16-byte pieces
     static_assert(T::WAVES * 16u * PITCH <= T::LDS, "the waves' rows fit the stages' place");
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* const own = lds + wave * 16u * PITCH;
     const bool pieces = (((uint64_t)a.ldy | n0) * sizeof(E) & 15u) == 0u && ((uintptr_t)a.y & 15u) == 0u;
 #pragma unroll
