@@ -300,6 +300,17 @@ def test_gemv(dev, m, n, k, ld, t):
 
 
 @pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
+@pytest.mark.parametrize("m,n,k", [(1, 40007, 64), (4, 17001, 544), (7, 9000, 2592), (16, 4500, 1056), (3, 5000, 3616), (2, 35, 33312), (1, 20, 90112)])
+def test_gemv_workgroups_with_several_tiles_and_long_rows(dev, t, m, n, k):
+    bank = random_bank(n, k, n)
+    wv, bufs = put_bank(dev, bank, k)
+    image, val = as_type(np.random.default_rng(m).standard_normal((m, k)), t)
+    _, y32 = gemv(dev, wv, image, t, m, n)
+    check_product(y32, val.astype(np.float64), bank[2], qwhip.F32)
+    free(*bufs)
+
+
+@pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
 @pytest.mark.parametrize("m", [1, 6])
 def test_gemv_scales_out_of_reach(dev, t, m):
     """Weights far outside f16's range meet small activations; NaN blocks show in their rows alone, also beside the end of a row."""
@@ -316,6 +327,23 @@ def test_gemv_scales_out_of_reach(dev, t, m):
     assert np.array_equal(np.isnan(y32), np.isnan(val.astype(np.float64) @ w.T))
     w[[9, 10]] = 0.0
     check_product(np.where(np.isnan(y32), 0.0, y32), val.astype(np.float64), w, qwhip.F32)
+    free(*bufs)
+
+
+@pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
+@pytest.mark.parametrize("byte", [0, 1, 2, 250, 252])
+def test_gemv_scales_at_the_ends(dev, t, byte):
+    """Every scale the smallest or the largest there is, with activations that bring the results back among fp32's normal numbers."""
+    n, k = 33, 672
+    bank = random_bank(n, k, 9)
+    scales = np.full_like(bank[1], byte)
+    image, val = as_type(np.random.default_rng(2).standard_normal((2, k)) * (2.0 ** 14 if byte < 100 else 2.0 ** -14), t)
+    wv, bufs = put_bank(dev, (bank[0], scales, None), k)
+    _, y32 = gemv(dev, wv, image, t, 2, n)
+    w, x = qwmx.values(bank[0], scales), val.astype(np.float64)
+    # a term under 2^-126 may lose what lies under 2^-149, half a step of fp32's subnormals, k of them
+    bound = (k + 32) * 2.0 ** -23 * (np.abs(x) @ np.abs(w).T) + k * 2.0 ** -149
+    assert (np.abs(y32 - x @ w.T) <= bound).all()
     free(*bufs)
 
 
