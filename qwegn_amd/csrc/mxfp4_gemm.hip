@@ -1,4 +1,6 @@
 // Product of two MXFP4 operands, Y[m, n] = X[m, k] . W[n, k]^T, on the scaled fp4 matrix instruction.
+#include <math.h>
+
 #include "qw_mxfp4.h"
 
 // ------------------------------------------------------------------------------------------------
@@ -14,13 +16,6 @@ struct qw_mx_operand {
     uint32_t rows, ld32;   // ld32: blocks from row to row
 };
 
-__device__ __forceinline__ void qw_mx_load(const qw_mx_operand& o, uint32_t row, uint32_t block, uint32_t blocks, u4_t& q, uint32_t& s) {
-    const uint64_t at = (uint64_t)min(row, o.rows - 1u) * o.ld32 + min(block, blocks - 1u);
-    q = *(const u4_t*)(o.codes + at * 16u);
-    s = o.scales[at];
-    if (block >= blocks) q = u4_t{0, 0, 0, 0}, s = 0;   // behind the last column: zeros under a finite scale
-}
-
 __device__ __forceinline__ f4_t qw_mx_mfma(u4_t a, uint32_t sa, u4_t b, uint32_t sb, f4_t c) {
     const i8_t av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
@@ -33,34 +28,65 @@ __device__ __forceinline__ void qw_mx_store(void* y, uint64_t at, float v) {
     else ((__bf16*)y)[at] = (__bf16)v;
 }
 
-// A wave: 32 x 32 of Y, operands straight from memory.
-template <int DT>
-__global__ __launch_bounds__(256) void qw_mx_gemm_plain_kernel(qw_mx_operand w, qw_mx_operand x, uint32_t blocks, void* __restrict__ y, uint32_t ldy) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i = lane & 15u, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 64u + (wave & 1u) * 32u, m0 = blockIdx.y * 64u + (wave >> 1) * 32u;
-    f4_t acc[2][2] = {};
-    for (uint32_t b = 0; b < blocks; b += 4u) {
-        u4_t qw[2], qx[2];
-        uint32_t sw[2], sx[2];
+// ------------------------------------------------------------------------------------------------
+// Few tiles: a workgroup owns 32 x 32 of Y and deals the columns to its waves in steps of 16 blocks (512 columns), operands straight from
+// memory; the waves' sums meet in LDS in the order of the waves.
+// ------------------------------------------------------------------------------------------------
+struct qw_mx_rows_load {   // a fragment's blocks g, 4 + g, 8 + g, 12 + g of a step and the step's scales of its row
+    u4_t q[4], sc;
+};
+__device__ __forceinline__ void qw_mx_rows_fetch(const uint8_t* codes, const uint8_t* scales, uint32_t b, uint32_t blocks, uint32_t g, qw_mx_rows_load& l) {
 #pragma unroll
-        for (uint32_t t = 0; t < 2; ++t) {
-            qw_mx_load(w, n0 + 16u * t + i, b + g, blocks, qw[t], sw[t]);
-            qw_mx_load(x, m0 + 16u * t + i, b + g, blocks, qx[t], sx[t]);
+    for (uint32_t u = 0; u < 4; ++u) l.q[u] = *(const u4_t*)(codes + (uint64_t)min(b + 4u * u + g, blocks - 1u) * 16u);
+    if (b + 16u <= blocks) {
+        __builtin_memcpy(&l.sc, scales + b, 16);
+    } else {   // behind the last block zeros: of both operands, so that what stands there adds 2^-254 times a finite code
+        l.sc = u4_t{0, 0, 0, 0};
+        for (uint32_t k = 0; k < 16u && b + k < blocks; ++k) {
+            const uint32_t v = (uint32_t)scales[b + k] << (8u * (k & 3u));
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) l.sc[u] |= (k >> 2) == u ? v : 0u;
         }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(1024) void qw_mx_gemm_rows_kernel(qw_mx_operand w, qw_mx_operand x, uint32_t blocks, void* __restrict__ y, uint32_t ldy) {
+    __shared__ f4_t part[16][4][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6, i = lane & 15u, g = lane >> 4;
+    const uint32_t n0 = blockIdx.x * 32u, m0 = blockIdx.y * 32u;
+    const uint8_t *codes[4], *scales[4];
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+    for (uint32_t f = 0; f < 4; ++f) {
+        const qw_mx_operand& o = f < 2u ? w : x;
+        const uint64_t row = (uint64_t)min((f < 2u ? n0 : m0) + 16u * (f & 1u) + i, o.rows - 1u) * o.ld32;
+        codes[f] = o.codes + row * 16u, scales[f] = o.scales + row;
+    }
+    f4_t acc[2][2] = {};
+    for (uint32_t b = wave * 16u; b < blocks; b += waves * 16u) {
+        qw_mx_rows_load l[4];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) acc[a][c] = qw_mx_mfma(qw[a], sw[a], qx[c], sx[c], acc[a][c]);
+        for (uint32_t f = 0; f < 4; ++f) qw_mx_rows_fetch(codes[f], scales[f], b, blocks, g, l[f]);
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) acc[a][c] = qw_mx_mfma(l[a].q[u], l[a].sc[u] >> (8u * g), l[2 + c].q[u], l[2 + c].sc[u] >> (8u * g), acc[a][c]);
     }
 #pragma unroll
-    for (uint32_t a = 0; a < 2; ++a)
+    for (int f = 0; f < 4; ++f) part[wave][f][lane] = acc[f >> 1][f & 1];
+    __syncthreads();
+    const uint32_t take = min(waves, 4u);   // the first waves sum the fragments
+    if (wave < take)
+        for (uint32_t f = wave; f < 4u; f += take) {
+            f4_t v = part[0][f][lane];
+            for (uint32_t p = 1; p < waves; ++p) v += part[p][f][lane];
+            const uint32_t n = n0 + 16u * (f >> 1) + 4u * g, m = m0 + 16u * (f & 1u) + i;
 #pragma unroll
-        for (uint32_t c = 0; c < 2; ++c)
-#pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                const uint32_t n = n0 + 16u * a + 4u * g + r, m = m0 + 16u * c + i;
-                if (n < w.rows && m < x.rows) qw_mx_store<DT>(y, (uint64_t)m * ldy + n, acc[a][c][r]);
-            }
+            for (uint32_t r = 0; r < 4; ++r)
+                if (n + r < w.rows && m < x.rows) qw_mx_store<DT>(y, (uint64_t)m * ldy + n + r, v[r]);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -93,6 +119,7 @@ struct qw_mx_tile_args {
     qw_mx_operand w, x;
     void* y;
     uint32_t blocks, ldy, tiles_m, tiles_n;
+    uint32_t range;   // stages of a K range (even), blockIdx.y its index: ranges write fp32 planes of m * ldy elements
 };
 
 template <int MF, int NF, int WM, int WN>
@@ -142,7 +169,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     }
 
     u4_t sstaged[T::SROWS];
-    const uint32_t stages = (a.blocks + 7u) / 8u;
+    const uint32_t begin = blockIdx.y * a.range, stages = min(begin + a.range, (a.blocks + 7u) / 8u);   // its stages: begin .. stages - 1
     // 1 KB of a stage from memory into LDS, eight rows of a wave: lane l's 16 bytes land at place l & 7 of row l >> 3
     auto fetch_codes = [&](uint32_t st, uint32_t into, auto j) {
         const uint32_t off = min(st * 8u + c, a.blocks - 1u) * 16u;   // behind the last block: any block, under scales of zero
@@ -161,10 +188,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
             for (uint32_t t = 0; t < T::SROWS; ++t)
 #pragma unroll
                 for (uint32_t q = 0; q < 4; ++q) {
-                    const uint32_t at = min(b + 4u * q, a.blocks - 4u), cut = 8u * (b + 4u * q - at);
-                    uint32_t v;
-                    __builtin_memcpy(&v, sbase[t] + (srow[t] + at), 4);
-                    sstaged[t][q] = cut < 32u ? v >> cut : 0u;
+                    uint32_t v = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        if (b + 4u * q + k < a.blocks) v |= (uint32_t)sbase[t][srow[t] + b + 4u * q + k] << (8u * k);
+                    sstaged[t][q] = v;
                 }
         }
     };
@@ -220,14 +248,14 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
         });
     };
 
-    fetch_scales(0);
-    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(0, 0, j); });
-    park_scales(0);
+    fetch_scales(begin >> 1);
+    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(begin, 0, j); });
+    park_scales(begin >> 1);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(1u, stages - 1u), 1, j); });
+    qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(begin + 1u, stages - 1u), 1, j); });
     constexpr std::integral_constant<int, 0> H0{};
     constexpr std::integral_constant<int, 1> H1{};
-    read_scales(0, H0);
+    read_scales(begin, H0);
     qw_static_for<MF>([&](auto j) { read_x(0, H0, j); });
     qw_static_for<NF>([&](auto j) { read_w(0, H0, j); });
     // A stage.  First half: its matrix instructions, the second half's fragments on their way in, the next stage into the other buffer.
@@ -267,7 +295,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    for (uint32_t st = 0; st < stages; st += 2u) {
+    for (uint32_t st = begin; st < stages; st += 2u) {
         stage(st, std::integral_constant<int, 0>{});
         if (st + 1u < stages) stage(st + 1u, std::integral_constant<int, 1>{});
     }
@@ -287,7 +315,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     const bool pieces = (((uint64_t)a.ldy | n0) * sizeof(E) & 15u) == 0u && ((uintptr_t)a.y & 15u) == 0u;
 #pragma unroll
     for (uint32_t m = 0; m < MF; ++m) {
-        E* const y = (E*)a.y + (uint64_t)(m0 + wm * 16u * MF + 16u * m) * a.ldy + (n0 + wn * 16u * NF);
+        E* const y = (E*)a.y + (uint64_t)blockIdx.y * a.x.rows * a.ldy + (uint64_t)(m0 + wm * 16u * MF + 16u * m) * a.ldy + (n0 + wn * 16u * NF);
 #pragma unroll
         for (uint32_t n = 0; n < NF; ++n) {
             const f4_t v = acc[n][m];
@@ -309,19 +337,82 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     }
 }
 
+// Sum of a product's planes in their order, four columns of a row a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void qw_mx_gemm_planes_kernel(const float* __restrict__ planes, uint32_t ranges, uint32_t m, uint32_t n, uint32_t pitch, void* __restrict__ y,
+                                                                 uint32_t ldy) {
+    const uint32_t quads = pitch / 4u;
+    const uint64_t id = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (id >= (uint64_t)m * quads) return;
+    const uint32_t row = (uint32_t)(id / quads), col = (uint32_t)(id - (uint64_t)row * quads) * 4u;
+    const float* from = planes + (uint64_t)row * pitch + col;
+    f4_t v = *(const f4_t*)from;
+    for (uint32_t r = 1; r < ranges; ++r) v += *(const f4_t*)(from + (uint64_t)r * m * pitch);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+        if (col + e < n) qw_mx_store<DT>(y, (uint64_t)row * ldy + col + e, v[e]);
+}
+
 template <int MF, int NF, int WM, int WN>
-static void qw_mx_launch_tile(qwhip_stream_t s, qw_mx_tile_args a, uint32_t y_dtype) {
+static void qw_mx_launch_tile(qwhip_stream_t s, qw_mx_tile_args a, uint32_t ranges, uint32_t y_dtype) {
     using T = qw_mx_tile<MF, NF, WM, WN>;
     a.tiles_m = qwhip_cdiv(a.x.rows, T::BM), a.tiles_n = qwhip_cdiv(a.w.rows, T::BN);
-    const dim3 grid(8u * qwhip_cdiv(a.tiles_m * a.tiles_n, 8u)), block(T::THREADS);
+    const dim3 grid(8u * qwhip_cdiv(a.tiles_m * a.tiles_n, 8u), ranges), block(T::THREADS);
     if (y_dtype == QWHIP_F32) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_F32>), grid, block, 0, s->stream, a);
     else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_F16>), grid, block, 0, s->stream, a);
     else hipLaunchKernelGGL((qw_mx_gemm_tile_kernel<MF, NF, WM, WN, QWHIP_BF16>), grid, block, 0, s->stream, a);
 }
 
+// The forms by what they cost, in microseconds, as measured: a tile on a compute unit `base + per_stage * stages`, where two fit a unit a
+// pair of them `base2 + per_stage2 * stages`; the rows kernel 3.5 and for a step (512 columns) 2.5e-3 a workgroup, 0.4 at least.  K ranges
+// add the sum's launch and its bytes at 3 TB/s, and run where that still pays: on few tiles of many columns.
+struct qw_mx_form {
+    uint32_t bm, bn, a_unit;
+    float base, per_stage, base2, per_stage2;
+};
+static const qw_mx_form g_mx_forms[] = {
+    {256, 256, 1, 5.0f, 1.65f, 0.0f, 0.0f},
+    {256, 192, 1, 4.5f, 1.45f, 0.0f, 0.0f},
+    {128, 128, 2, 5.0f, 0.8f, 6.0f, 1.1f},
+    {64, 128, 2, 5.0f, 0.65f, 6.0f, 0.75f},
+};
+constexpr uint32_t QW_MX_FORMS = 4, QW_MX_ROWS_FORM = QW_MX_FORMS;
+static void qw_mx_launch_form(qwhip_stream_t s, uint32_t form, const qw_mx_tile_args& a, uint32_t ranges, uint32_t y_dtype) {
+    if (form == 0u) qw_mx_launch_tile<4, 8, 4, 2>(s, a, ranges, y_dtype);
+    else if (form == 1u) qw_mx_launch_tile<4, 6, 4, 2>(s, a, ranges, y_dtype);
+    else if (form == 2u) qw_mx_launch_tile<2, 4, 4, 2>(s, a, ranges, y_dtype);
+    else qw_mx_launch_tile<1, 4, 4, 2>(s, a, ranges, y_dtype);
+}
+
+struct qw_mx_plan {
+    uint32_t form, ranges, range;
+};
+static uint32_t qw_mx_pitch(uint32_t n) { return (n + 3u) & ~3u; }   // of a plane
+static qw_mx_plan qw_mx_choose(uint32_t m, uint32_t n, uint32_t blocks, bool tiles_ok, uint64_t room) {
+    const uint32_t stages = qwhip_cdiv(blocks, 8u), steps = qwhip_cdiv(blocks, 16u);
+    qw_mx_plan best = {QW_MX_ROWS_FORM, 1u, 0u};
+    float least = 3.5f + (float)steps * fmaxf(0.4f, 2.5e-3f * (float)qwhip_cdiv(n, 32u) * (float)qwhip_cdiv(m, 32u));
+    for (uint32_t f = 0; f < QW_MX_FORMS && tiles_ok; ++f) {
+        const qw_mx_form& t = g_mx_forms[f];
+        if (m < t.bm || n < t.bn) continue;
+        const uint64_t tiles = (uint64_t)qwhip_cdiv(m, t.bm) * qwhip_cdiv(n, t.bn), plane = (uint64_t)m * qw_mx_pitch(n) * 4u;
+        for (uint32_t want = 1; want <= 16u; ++want) {
+            const uint32_t range = (qwhip_cdiv(stages, want) + 1u) & ~1u, ranges = qwhip_cdiv(stages, range);   // whole steps of scales
+            if (want > 1u && (ranges != want || ranges * plane > room || tiles * ranges > 512u)) continue;
+            const uint64_t a_unit = (tiles * ranges + 255u) / 256u;
+            const float one = t.base + t.per_stage * (float)range, two = t.base2 + t.per_stage2 * (float)range;
+            float cost = t.a_unit == 1u ? (float)a_unit * one : (float)(a_unit / 2u) * two + (float)(a_unit % 2u) * one;
+            if (ranges > 1u) cost += 1.5f + ((float)ranges + 0.5f) * (float)plane / 3e6f;
+            if (cost < least) least = cost, best = {f, ranges, range};
+        }
+    }
+    return best;
+}
+
 extern "C" uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
-    (void)m, (void)n, (void)k;
-    return 0;
+    if (m == 0 || n == 0 || k == 0 || k % 32u != 0) return 0;
+    const qw_mx_plan plan = qw_mx_choose(m, n, k / 32u, true, ~(uint64_t)0);
+    return plan.ranges > 1u ? (uint64_t)plan.ranges * m * qw_mx_pitch(n) * 4u : 0u;
 }
 
 extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const qwhip_mxfp4_view* x, void* y, uint32_t y_dtype, uint32_t ldy,
@@ -342,19 +433,31 @@ extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_vie
     if (ldy < w->n) return qwhip_fail(QWHIP_E_BAD_SHAPE, "output row pitch %u is under n=%u", ldy, w->n);
     if ((uintptr_t)y & (y_dtype == QWHIP_F32 ? 3u : 1u)) return qwhip_fail(QWHIP_E_BAD_SHAPE, "GEMM output is not aligned to its elements");
     if ((uintptr_t)workspace & 15u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "GEMM workspace must be 16-byte aligned");
-    if (x->n > 65535u * 64u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows do not fit one launch", x->n);
+    if (x->n > 65535u * 32u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows do not fit one launch", x->n);
     QW_ON_DEVICE_OF(s);
     const qw_mx_operand ow = {(const uint8_t*)w->codes, (const uint8_t*)w->scales, w->n, qw_mxfp4_ld(w) / 32u};
     const qw_mx_operand ox = {(const uint8_t*)x->codes, (const uint8_t*)x->scales, x->n, qw_mxfp4_ld(x) / 32u};
-    if (x->n >= 256u && w->n >= 256u && w->k >= 128u && ow.ld32 < (1u << 18) && ox.ld32 < (1u << 18)) {   // 32-bit offsets inside a tile
-        qw_mx_launch_tile<4, 8, 4, 2>(s, {ow, ox, y, w->k / 32u, ldy, 0, 0}, y_dtype);
-        QWHIP_TRY_HIP(hipGetLastError());
-        return QWHIP_OK;
+    const uint32_t blocks = w->k / 32u;
+    const bool tiles_ok = ow.ld32 < (1u << 18) && ox.ld32 < (1u << 18);   // 32-bit offsets inside a tile
+    const qw_mx_plan plan = qw_mx_choose(x->n, w->n, blocks, tiles_ok, workspace ? workspace_bytes : 0u);
+    if (plan.ranges > 1u) {
+        const uint32_t pitch = qw_mx_pitch(w->n);
+        qw_mx_launch_form(s, plan.form, {ow, ox, workspace, blocks, pitch, 0, 0, plan.range}, plan.ranges, QWHIP_F32);
+        const dim3 grid((unsigned)(((uint64_t)x->n * (pitch / 4u) + 255u) / 256u)), block(256);
+#define QW_MX_PLANES(DT) \
+    hipLaunchKernelGGL(qw_mx_gemm_planes_kernel<DT>, grid, block, 0, s->stream, (const float*)workspace, plan.ranges, x->n, w->n, pitch, y, ldy)
+        if (y_dtype == QWHIP_F32) QW_MX_PLANES(QWHIP_F32);
+        else if (y_dtype == QWHIP_F16) QW_MX_PLANES(QWHIP_F16);
+        else QW_MX_PLANES(QWHIP_BF16);
+#undef QW_MX_PLANES
+    } else if (plan.form != QW_MX_ROWS_FORM) {
+        qw_mx_launch_form(s, plan.form, {ow, ox, y, blocks, ldy, 0, 0, plan.range}, 1, y_dtype);
+    } else {
+        const dim3 grid(qwhip_cdiv(w->n, 32u), qwhip_cdiv(x->n, 32u)), block(64u * min(16u, qwhip_cdiv(blocks, 16u)));
+        if (y_dtype == QWHIP_F32) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F32>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
+        else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F16>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
+        else hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_BF16>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
     }
-    const dim3 grid(qwhip_cdiv(w->n, 64u), qwhip_cdiv(x->n, 64u)), block(256);
-    if (y_dtype == QWHIP_F32) hipLaunchKernelGGL(qw_mx_gemm_plain_kernel<QWHIP_F32>, grid, block, 0, s->stream, ow, ox, w->k / 32u, y, ldy);
-    else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL(qw_mx_gemm_plain_kernel<QWHIP_F16>, grid, block, 0, s->stream, ow, ox, w->k / 32u, y, ldy);
-    else hipLaunchKernelGGL(qw_mx_gemm_plain_kernel<QWHIP_BF16>, grid, block, 0, s->stream, ow, ox, w->k / 32u, y, ldy);
     QWHIP_TRY_HIP(hipGetLastError());
     return QWHIP_OK;
 }

@@ -195,7 +195,9 @@ def gemm(dev, wv, xv, m, n, t, ldy=0, workspace=None, stream=None):
 
 
 GEMM_SHAPES = [(1, 1, 32), (1, 640, 1024), (16, 640, 1024), (3, 17, 64), (77, 1003, 1056), (64, 256, 128), (129, 130, 160), (255, 257, 96), (257, 511, 1312), (256, 256, 5120),
-               (512, 768, 512), (300, 4099, 288), (33, 48, 17408), (1000, 320, 2080), (700, 1028, 544), (513, 1030, 768), (260, 516, 2048), (2, 5120, 640), (40, 2560, 992)]
+               (512, 768, 512), (300, 4099, 288), (33, 48, 17408), (1000, 320, 2080), (700, 1028, 544), (513, 1030, 768), (260, 516, 2048), (2, 5120, 640), (40, 2560, 992),
+               # whole and half tiles, edges that overlap, K ranges (with a workspace), columns that end inside a stage
+               (64, 128, 32), (70, 200, 96), (1000, 1000, 1024), (2048, 5100, 288), (6000, 5000, 96), (200, 650, 17408), (520, 517, 9632), (8026, 300, 64)]
 
 
 @pytest.mark.parametrize("m,n,k", GEMM_SHAPES)
