@@ -113,6 +113,14 @@ __device__ __forceinline__ void qw_mx_mfma_at(u4_t a, uint32_t sa, u4_t b, uint3
                  : "+a"(c)
                  : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(OA & 1), "n"(OB & 1), "n"(OA >> 1), "n"(OB >> 1));
 }
+// All of a wave's loads and LDS accesses done, then the workgroup's; by builtins, so that the compiler knows that nothing is left to wait for.
+#define QW_MX_BARRIER()                                          \
+    do {                                                         \
+        asm volatile("" ::: "memory");                           \
+        __builtin_amdgcn_s_waitcnt(0x0070); /* vmcnt, lgkmcnt */ \
+        __builtin_amdgcn_s_barrier();                            \
+        asm volatile("" ::: "memory");                           \
+    } while (0)
 #define QW_MX_DRAIN() asm volatile("s_nop 15\n\ts_nop 15" ::: "memory")   // more wait states than a matrix instruction's result takes
 
 struct qw_mx_tile_args {
@@ -251,7 +259,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     fetch_scales(begin >> 1);
     qw_static_for<T::PIECES>([&](auto j) { fetch_codes(begin, 0, j); });
     park_scales(begin >> 1);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch_scales(min((begin >> 1) + 1u, (stages - 1u) >> 1));
+    QW_MX_BARRIER();
     qw_static_for<T::PIECES>([&](auto j) { fetch_codes(min(begin + 1u, stages - 1u), 1, j); });
     constexpr std::integral_constant<int, 0> H0{};
     constexpr std::integral_constant<int, 1> H1{};
@@ -265,33 +274,34 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     auto stage = [&](uint32_t st, auto parity) {
         constexpr int P = decltype(parity)::value;
         const uint32_t after = min(st + 2u, stages - 1u), step = st >> 1;
-        read_scales(st, H1);
-        if constexpr (P == 0) fetch_scales(min(step + 1u, (stages - 1u) >> 1));
         qw_static_for<NF>([&](auto n) {
             constexpr int N = decltype(n)::value;
+            multiply(H0, n);
+            if constexpr (N == 0) read_scales(st, H1);
             qw_static_for<PERX>([&](auto k) {
                 constexpr int J = N * PERX + decltype(k)::value;
                 if constexpr (J < MF) read_x(st, H1, std::integral_constant<int, J>{});
             });
-            if constexpr (P == 1 && N == NF / 2) park_scales(step + 1u);
-            multiply(H0, n);
             read_w(st, H1, n);
             __builtin_amdgcn_sched_barrier(0);
         });
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        read_scales(st + 1u, H0);
+        QW_MX_BARRIER();
         qw_static_for<NF>([&](auto n) {
             constexpr int N = decltype(n)::value;
+            multiply(H1, n);
+            if constexpr (N == 0) read_scales(st + 1u, H0);
             qw_static_for<PERX>([&](auto k) {
                 constexpr int J = N * PERX + decltype(k)::value;
                 if constexpr (J < MF) read_x(st + 1u, H0, std::integral_constant<int, J>{});
             });
+            read_w(st + 1u, H0, n);
+            // scales: asked for a step ahead, into LDS here, where no load is under way (a store to LDS waits for the ones into it)
+            if constexpr (P == 0 && N == 0) park_scales(step + 1u);
+            if constexpr (P == 1 && N == 0) fetch_scales(min(step + 2u, (stages - 1u) >> 1));
             qw_static_for<PER>([&](auto k) {
                 constexpr int J = N * PER + decltype(k)::value;
                 if constexpr (J < (int)T::PIECES) fetch_codes(after, st, std::integral_constant<int, J>{});
             });
-            multiply(H1, n);
-            read_w(st + 1u, H0, n);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void qw_mx_gemm_tile_ker
     typedef E e4_t __attribute__((ext_vector_type(4)));
     constexpr uint32_t PITCH = 16u * NF * sizeof(E) + 16u, ROW16 = NF * sizeof(E);   // bytes of a row in LDS; its 16-byte pieces
     static_assert(T::WAVES * 16u * PITCH <= T::LDS, "the waves' rows fit the stages' place");
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    QW_MX_BARRIER();
     uint8_t* const own = lds + wave * 16u * PITCH;
     const bool pieces = (((uint64_t)a.ldy | n0) * sizeof(E) & 15u) == 0u && ((uintptr_t)a.y & 15u) == 0u;
 #pragma unroll
