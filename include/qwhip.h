@@ -558,23 +558,24 @@ qwhip_status qwhip_mxfp4_view_validate(const qwhip_mxfp4_view* v);
  * 2^(floor(log2 max|v|) - 2), at least 2^-127; an element is the nearest e2m1 value of v / scale, ties to the even code,
  * magnitudes over 6 to 6, the sign kept.  A block with an infinity or a NaN gets scale byte 255 and codes 0 (it reads as NaN).
  * values (may be NULL; 16-byte aligned): what the codes stand for, [rows, k] tight in src's type, exact; codes and values 16-byte
- * aligned.  src, codes, scales and values do not overlap. */
+ * aligned.  src, codes, scales and values do not overlap; rows * k < 2^35. */
 qwhip_status qwhip_quantize_mxfp4(qwhip_stream_t s, const void* src, uint32_t src_dtype, uint32_t rows, uint32_t k, uint32_t ld,
                                   void* codes, void* scales, void* values);
 /* out [n, k] row-major, tight, 16-byte aligned: the values of a bank; exact in f32 and bf16 (from 2^128 on,
- * which scale bytes 253 and 254 reach, infinity), rounded where f16 does not hold them. */
+ * which scale bytes 253 and 254 reach, infinity), rounded where f16 does not hold them; n * k < 2^35. */
 qwhip_status qwhip_dequant_mxfp4(qwhip_stream_t s, const qwhip_mxfp4_view* v, void* out, uint32_t out_dtype);
 /* y [m, n] = X . W^T of two quantised operands, w [n, k] and x [m = x->n, k], any m (0 rows: nothing to do), n and k % 32 == 0; y f32,
  * f16 or bf16 with row pitch ldy elements (0 = n).  fp32 accumulation of exact products, one rounding at the store.
  * workspace (may be NULL; 16-byte aligned) lets few tiles split k over more compute units: fp32 planes of m * n elements, at
  * most qwhip_mxfp4_gemm_workspace_bytes(m, n, k) bytes of it.  The planes are summed in a fixed order; which form runs
  * follows from m, n, k, the pitches and the room in the workspace, never from its contents.  Two calls that overlap in time
- * take two workspaces. */
+ * take two workspaces.  y and the workspace do not overlap the operands; a NaN block makes its row or column of y NaN. */
 qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const qwhip_mxfp4_view* x, void* y, uint32_t y_dtype,
                               uint32_t ldy, void* workspace, uint64_t workspace_bytes);
 uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
 /* Decode / verify: y [m, n] = x . W^T for m = 1..16 rows (0: nothing to do) of f16 or bf16 activations [m, k], tight and 16-byte
- * aligned, not quantised; y16 (f16) and / or y32 (f32), at least one.  Every weight byte is read once for all rows; fp32 accumulation. */
+ * aligned, not quantised; y16 (f16) and / or y32 (f32), at least one.  Every weight byte is read once for all rows; fp32 accumulation
+ * in an order that follows from m, n, k and, for f16, from the scales. */
 qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_view* w, const void* x, uint32_t x_dtype, uint32_t m, void* y16,
                               float* y32);
 

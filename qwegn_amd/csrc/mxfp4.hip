@@ -124,7 +124,7 @@ extern "C" qwhip_status qwhip_quantize_mxfp4(qwhip_stream_t s, const void* src, 
     if (((uintptr_t)src & 15u) || ((uintptr_t)codes & 15u) || ((uintptr_t)values & 15u))
         return qwhip_fail(QWHIP_E_BAD_SHAPE, "quantizer needs a 16-byte aligned source, codes and values");
     const uint64_t pieces = (uint64_t)rows * (k / 8u);
-    if (pieces > (uint64_t)0x7FFFFFFFu * 256u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of %u columns do not fit one launch", rows, k);
+    if (pieces > 0xFFFFFF00u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of %u columns do not fit one launch", rows, k);
     QW_ON_DEVICE_OF(s);
     if (rows == 1) ld = k;
     if (src_dtype == QWHIP_F32) qw_launch_quantize_mxfp4<QWHIP_F32>(s, src, (uint32_t*)codes, (uint8_t*)scales, values, pieces, k / 8u, ld);
@@ -161,7 +161,7 @@ extern "C" qwhip_status qwhip_dequant_mxfp4(qwhip_stream_t s, const qwhip_mxfp4_
     if (out_dtype != QWHIP_F32 && out_dtype != QWHIP_F16 && out_dtype != QWHIP_BF16)
         return qwhip_fail(QWHIP_E_BAD_SHAPE, "dequant output must be f32, f16 or bf16, got dtype %u", out_dtype);
     const uint64_t pieces = (uint64_t)v->n * (v->k / 8u);
-    if (pieces > (uint64_t)0x7FFFFFFFu * 256u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of %u columns do not fit one launch", v->n, v->k);
+    if (pieces > 0xFFFFFF00u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of %u columns do not fit one launch", v->n, v->k);
     QW_ON_DEVICE_OF(s);
     const dim3 grid((unsigned)((pieces + 255u) / 256u)), block(256);
     const uint32_t ld = v->n == 1 ? v->k : qw_mxfp4_ld(v);

@@ -41,12 +41,14 @@ __device__ __forceinline__ f4_t qw_mfma16(u4_t a, u4_t b, f4_t c) {
 // that row, a step ahead of their use.
 // bf16: the scaled elements are bf16 numbers, so a lane turns its block into four operands and the matrix unit contracts them with the
 // same columns of x.
-// f16: scales reach far outside of f16, so the codes go in unscaled.  A transpose over the lane rows leaves a lane eight codes of each of
-// four blocks; a matrix instruction then contracts one block, and the block's scale multiplies its fp32 sums.
+// f16: so they are for scales of 2^-13 .. 2^13, whose elements are normal f16 numbers; where a wave's step has all of its scales there, it is
+// taken the same way.  Other scales: the codes go in unscaled.  A transpose over the lane rows leaves a lane eight codes of each of four
+// blocks; a matrix instruction then contracts one block, and the block's scale multiplies its fp32 sums.  (A block's instructions: 22 the
+// first way, 54 the second.)
 // Bound by the weights' bytes on long banks (151936 x 5120, one row: 75 us = 5.5 TB/s, at the rate of a large copy), by start and end of the
 // launch on shorter ones (17408 x 5120: 12.1 us = 3.9 TB/s).  x straight from memory instead of LDS, four of its lines for one of weights,
-// took 14.7 and 114 us.  Eight f16 rows of 17408 columns pass x through LDS once for 32 weight rows: 19.8 us, 15.6 without reading x.
-constexpr uint32_t QW_MX_GEMV_STEP = 16, QW_MX_GEMV_AHEAD = 4;
+// took 14.7 and 114 us.  Eight f16 rows of 17408 columns pass x through LDS once for 32 weight rows: 17.6 us (19.3 with every step unscaled).
+constexpr uint32_t QW_MX_GEMV_STEP = 16, QW_MX_GEMV_AHEAD = 4, QW_MX_F16_LEAST = 114, QW_MX_F16_MOST = 140;
 struct qw_mx_gemv_load {   // what a lane carries of a step of weights
     u4_t q[4], sc;
 };
@@ -76,24 +78,37 @@ __device__ __forceinline__ float qw_mx_scale(uint32_t word, uint32_t shift) {
 // `xrow`: row i of x in LDS from the step's first column on.
 template <int DT>
 __device__ __forceinline__ void qw_mx_gemv_multiply(const qw_mx_gemv_load& l, const uint8_t* xrow, uint32_t g, f4_t (&acc)[2]) {
+    uint32_t byte[4];
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-        if constexpr (DT == QWHIP_BF16) {
-            const float s = __uint_as_float(((l.sc[u] >> (8u * g)) & 0xFFu) << 23);
+    for (uint32_t u = 0; u < 4; ++u) byte[u] = (l.sc[u] >> (8u * g)) & 0xFFu;
+    bool scaled = true;
+    if constexpr (DT == QWHIP_F16) {
+        uint32_t far = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) far = max(far, byte[u] - QW_MX_F16_LEAST);
+        scaled = __ballot(far > QW_MX_F16_MOST - QW_MX_F16_LEAST) == 0ull;
+    }
+    if (scaled) {
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const float s = __uint_as_float(byte[u] << 23);
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)   // columns 8 j .. of the lane's own block
                 acc[j & 1] = qw_mfma16<DT>(*(const u4_t*)(xrow + (4u * u + g) * 64u + 16u * j), qw_e2m1_operand<DT>(l.q[u][j], s), acc[j & 1]);
-        } else {
-            uint32_t q0 = l.q[u][0], q1 = l.q[u][1], q2 = l.q[u][2], q3 = l.q[u][3];
-            qw_transpose_rows4(q0, q1, q2, q3);
-            const uint32_t own[4] = {q0, q1, q2, q3};
+        }
+        return;
+    }
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {   // columns 8 g .. of block j
-                const f4_t d = qw_mfma16<DT>(*(const u4_t*)(xrow + (4u * u + j) * 64u + 16u * g), qw_e2m1_operand<DT>(own[j], 1.0f), f4_t{0.f, 0.f, 0.f, 0.f});
-                const float s = qw_mx_scale(l.sc[u], 8u * j);
+    for (uint32_t u = 0; u < 4; ++u) {
+        uint32_t q0 = l.q[u][0], q1 = l.q[u][1], q2 = l.q[u][2], q3 = l.q[u][3];
+        qw_transpose_rows4(q0, q1, q2, q3);
+        const uint32_t own[4] = {q0, q1, q2, q3};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[j & 1][r] = __builtin_fmaf(s, d[r], acc[j & 1][r]);
-            }
+        for (uint32_t j = 0; j < 4; ++j) {   // columns 8 g .. of block j
+            const f4_t d = qw_mfma16<DT>(*(const u4_t*)(xrow + (4u * u + j) * 64u + 16u * g), qw_e2m1_operand<DT>(own[j], 1.0f), f4_t{0.f, 0.f, 0.f, 0.f});
+            const float s = qw_mx_scale(l.sc[u], 8u * j);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j & 1][r] = __builtin_fmaf(s, d[r], acc[j & 1][r]);
         }
     }
 }
@@ -200,8 +215,8 @@ extern "C" qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_vie
     QW_ON_DEVICE_OF(s);
     const uint32_t blocks = w->k / 32u, tiles = qwhip_cdiv(w->n, 16u), steps = qwhip_cdiv(blocks, QW_MX_GEMV_STEP);
     // 16 waves a compute unit carry what its memory pipe needs in flight: in four workgroups where four copies of x and of the sums fit its
-    // LDS, in two, in one (rows of 5120, 17408 outputs, one row: 12.1 / 12.6 / 13.2 us with 4 / 8 / 16 ways; 17408 -> 5120: 17.9 / 16.7 / 18.1;
-    // eight rows of 5120: 45.4 / 25.5 / 18.8).  Past that x passes through LDS in chunks of a step a way, the next one carried in registers.
+    // LDS, in two, in one (rows of 5120, 17408 outputs, one row: 12.1 / 12.5 / 13.5 us with 4 / 8 / 16 ways; 17408 -> 5120: 14.6 / 14.1 / 15.2;
+    // eight rows of 5120: 39.4 / 16.3 / 16.3).  Past that x passes through LDS in chunks of a step a way, the next one carried in registers.
     const uint64_t row = (uint64_t)steps * 1024u + 16u, lds_bytes = 160u << 10;
     uint64_t lds = 0;
     uint32_t row_tiles = 1, ways = 4, chunk = steps, chunks = 1;

@@ -349,6 +349,47 @@ def test_gemv_scales_at_the_ends(dev, t, byte):
     free(*bufs)
 
 
+@pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
+@pytest.mark.parametrize("byte", [113, 114, 140, 141])
+def test_gemv_scales_about_the_normal_f16_numbers(dev, t, byte):
+    """Scales whose elements begin or cease to be normal f16 numbers, alone and mixed with others inside steps, rows and waves."""
+    n, k = 50, 2336
+    bank = random_bank(n, k, 19)
+    scales = np.full_like(bank[1], byte)
+    scales[17:30, ::5] = 121
+    scales[30:, 40:] = 127
+    scales[40, 3] = 90
+    image, val = as_type(np.random.default_rng(3).standard_normal((3, k)), t)
+    wv, bufs = put_bank(dev, (bank[0], scales, None), k)
+    _, y32 = gemv(dev, wv, image, t, 3, n)
+    check_product(y32, val.astype(np.float64), qwmx.values(bank[0], scales), qwhip.F32)
+    free(*bufs)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 700, 1056), (5, 333, 2592), (16, 96, 17408), (8, 200, 9216)])
+def test_gemv_f16_scales_in_and_out_of_range(dev, m, n, k):
+    bank = random_bank(n, k, m, spread=9)                       # 2^-15 .. 2^3: some steps of a wave are in range, some are not
+    bank[1][: n // 2] = np.maximum(bank[1][: n // 2], 114)
+    w = qwmx.values(bank[0], bank[1])
+    wv, bufs = put_bank(dev, bank, k)
+    image, val = as_type(np.random.default_rng(m).standard_normal((m, k)), qwhip.F16)
+    _, y32 = gemv(dev, wv, image, qwhip.F16, m, n)
+    check_product(y32, val.astype(np.float64), w, qwhip.F32)
+    free(*bufs)
+
+
+@pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
+def test_gemv_small_activations(dev, t):
+    """Activations among the subnormal numbers of f16."""
+    n, k, m = 64, 1120, 4
+    bank = random_bank(n, k, 23)
+    image, val = as_type(np.random.default_rng(4).standard_normal((m, k)) * 2.0 ** -17, t)
+    wv, bufs = put_bank(dev, bank, k)
+    _, y32 = gemv(dev, wv, image, t, m, n)
+    check_product(y32, val.astype(np.float64), bank[2], qwhip.F32)
+    free(*bufs)
+
+
 def test_gemv_captured(dev):
     n, k, m = 640, 2048, 3
     bank = random_bank(n, k, 6)

@@ -41,7 +41,7 @@ def test_view(lib):
     (dict(k=0), qwhip.E_BAD_SHAPE), (dict(k=40), qwhip.E_BAD_SHAPE), (dict(ld=32), qwhip.E_BAD_SHAPE), (dict(ld=66), qwhip.E_BAD_SHAPE),
     (dict(t=qwhip.F32, ld=66), qwhip.E_BAD_SHAPE), (dict(ld=68), qwhip.E_BAD_SHAPE), (dict(t=qwhip.I32), qwhip.E_BAD_SHAPE), (dict(t=9), qwhip.E_BAD_SHAPE),
     (dict(src=BASE + 8), qwhip.E_BAD_SHAPE), (dict(codes=BASE + 4), qwhip.E_BAD_SHAPE), (dict(values=BASE + 2), qwhip.E_BAD_SHAPE),
-    (dict(rows=0xFFFFFFFF, k=0xFFFFFFE0), qwhip.E_BAD_SHAPE), (dict(rows=0), qwhip.OK), (dict(rows=0, src=None), qwhip.OK)])
+    (dict(rows=0xFFFFFFFF, k=0xFFFFFFE0), qwhip.E_BAD_SHAPE), (dict(rows=1 << 20, k=1 << 15), qwhip.E_BAD_SHAPE), (dict(rows=0), qwhip.OK), (dict(rows=0, src=None), qwhip.OK)])
 def test_quantise(lib, change, want):
     a = dict(s=ST, src=BASE, t=qwhip.F16, rows=4, k=64, ld=0, codes=BASE + 4096, scales=BASE + 8192, values=BASE + 16384) | change
     assert lib.qwhip_quantize_mxfp4(a["s"], a["src"], a["t"], a["rows"], a["k"], a["ld"], a["codes"], a["scales"], a["values"]) == want
@@ -55,6 +55,7 @@ def test_dequant(lib):
     assert lib.qwhip_dequant_mxfp4(ST, C.byref(v), BASE + 4, 0) == qwhip.E_BAD_SHAPE
     assert lib.qwhip_dequant_mxfp4(ST, C.byref(v), BASE, 3) == qwhip.E_BAD_SHAPE
     assert lib.qwhip_dequant_mxfp4(ST, C.byref(view(k=33)), BASE, 0) == qwhip.E_BAD_WEIGHTS
+    assert lib.qwhip_dequant_mxfp4(ST, C.byref(view(n=1 << 20, k=1 << 15, cb=1 << 40, sb=1 << 40)), BASE, 0) == qwhip.E_BAD_SHAPE
 
 
 @pytest.mark.parametrize("change,want", [
