@@ -122,6 +122,7 @@ struct qw_mx_gemv_args {
     uint32_t n, blocks, ld32, m;
     uint32_t row_tiles, ways;   // waves of a workgroup: row_tiles tiles of 16 weight rows x ways ranges of the columns
     uint32_t chunk, chunks;     // steps of x that LDS holds at a time; how many times
+    uint32_t group;             // rows of x that a workgroup takes, blockIdx.y its group
 };
 
 template <int DT, bool CHUNKED>
@@ -129,17 +130,19 @@ __global__ __launch_bounds__(1024) void qw_mx_gemv_kernel(const qw_mx_gemv_args 
     extern __shared__ __attribute__((aligned(16))) uint8_t qw_gemv_lds[];
     const uint32_t tid = threadIdx.x, threads = blockDim.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), i = lane & 15u, g = lane >> 4;
     const uint32_t rt = wave / a.ways, way = wave - rt * a.ways, waves = a.row_tiles * a.ways;
-    const uint32_t pitch = a.chunk * 1024u + 16u, buffer = a.m * pitch;   // rows 16 bytes on in the banks
+    const uint32_t row_first = blockIdx.y * a.group, m = min(a.group, a.m - row_first);
+    const uint16_t* const xg = a.x + (uint64_t)row_first * a.blocks * 32u;
+    const uint32_t pitch = a.chunk * 1024u + 16u, buffer = m * pitch;   // rows 16 bytes on in the banks
     f4_t* const part = (f4_t*)(qw_gemv_lds + (CHUNKED ? 2u : 1u) * buffer);
-    const uint8_t* const xlds = qw_gemv_lds + min(i, a.m - 1u) * pitch;   // rows behind the last one: sums that are not stored
+    const uint8_t* const xlds = qw_gemv_lds + min(i, m - 1u) * pitch;   // rows behind the last one: sums that are not stored
     const uint32_t steps = (a.blocks + QW_MX_GEMV_STEP - 1u) / QW_MX_GEMV_STEP, tiles = (a.n + 15u) / 16u;
 
     // chunk ch of x: pieces of eight columns, zeros behind the last column
-    const uint32_t row_pieces = a.chunk * 64u, pieces = a.m * row_pieces;
+    const uint32_t row_pieces = a.chunk * 64u, pieces = m * row_pieces;
     auto piece = [&](uint32_t ch, uint32_t p) {
         const uint32_t row = p / row_pieces, col = p - row * row_pieces + ch * row_pieces;
         u4_t v = {0, 0, 0, 0};
-        if (p < pieces && col < a.blocks * 4u) v = *(const u4_t*)(a.x + ((uint64_t)row * a.blocks * 32u + col * 8u));
+        if (p < pieces && col < a.blocks * 4u) v = *(const u4_t*)(xg + ((uint64_t)row * a.blocks * 32u + col * 8u));
         return v;
     };
     auto place = [&](uint32_t ch, uint32_t p, u4_t v) {
@@ -191,9 +194,9 @@ __global__ __launch_bounds__(1024) void qw_mx_gemv_kernel(const qw_mx_gemv_args 
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r) {
                 const uint32_t t = 4u * g + r;
-                if (col < a.n && t < a.m) {
-                    if (a.y16) a.y16[(uint64_t)t * a.n + col] = (h1_t)acc[0][r];
-                    if (a.y32) a.y32[(uint64_t)t * a.n + col] = acc[0][r];
+                if (col < a.n && t < m) {
+                    if (a.y16) a.y16[(uint64_t)(row_first + t) * a.n + col] = (h1_t)acc[0][r];
+                    if (a.y32) a.y32[(uint64_t)(row_first + t) * a.n + col] = acc[0][r];
                 }
             }
         }
@@ -219,22 +222,25 @@ extern "C" qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_vie
     // eight rows of 5120: 39.4 / 16.3 / 16.3).  Past that x passes through LDS in chunks of a step a way, the next one carried in registers.
     const uint64_t row = (uint64_t)steps * 1024u + 16u, lds_bytes = 160u << 10;
     uint64_t lds = 0;
-    uint32_t row_tiles = 1, ways = 4, chunk = steps, chunks = 1;
+    uint32_t row_tiles = 1, ways = 4, chunk = steps, chunks = 1, group = m;
     for (; ways <= 16u; ways *= 2u) {
         lds = m * row + 2u * min(ways, steps) * 1024u;
         if (lds * (16u / ways) <= lds_bytes) break;
     }
     const bool chunked = ways > 16u;
     if (chunked) {
-        row_tiles = m > 8u ? 4u : 2u, ways = 16u / row_tiles;
+        // nine and more rows: four tiles a workgroup, unless that leaves most units idle: then two groups of rows, each with the weights
+        // (11 rows of 8768 on 2116 outputs, 34 workgroups of four tiles: 17.8 -> 12.2 us; 16 rows of 17408 on 5120, 80 of them: 32.3 -> 34.5)
+        if (m > 8u && qwhip_cdiv(tiles, 4u) < 64u) group = (m + 1u) / 2u;
+        row_tiles = group > 8u ? 4u : 2u, ways = 16u / row_tiles;
         chunk = ways, chunks = qwhip_cdiv(steps, chunk);
-        lds = 2u * m * (chunk * 1024u + 16u) + 16u * 1024u;   // at most 144 KB
+        lds = 2u * group * (chunk * 1024u + 16u) + 16u * 1024u;   // at most 144 KB
     }
     const uint32_t resident = chunked ? tiles : 256u * 16u / ways;   // a workgroup keeps x and walks over tiles
     ways = min(ways, steps);
     const qw_mx_gemv_args a = {(const uint8_t*)w->codes, (const uint8_t*)w->scales, (const uint16_t*)x, (h1_t*)y16, y32, w->n, blocks, qw_mxfp4_ld(w) / 32u, m,
-                               row_tiles, ways, chunk, chunks};
-    const dim3 grid(min(qwhip_cdiv(tiles, row_tiles), resident)), block(64u * row_tiles * ways);
+                               row_tiles, ways, chunk, chunks, group};
+    const dim3 grid(min(qwhip_cdiv(tiles, row_tiles), resident), qwhip_cdiv(m, group)), block(64u * row_tiles * ways);
     void (*const kernel)(qw_mx_gemv_args) = x_dtype == QWHIP_F16 ? (chunked ? qw_mx_gemv_kernel<QWHIP_F16, true> : qw_mx_gemv_kernel<QWHIP_F16, false>)
                                                                   : (chunked ? qw_mx_gemv_kernel<QWHIP_BF16, true> : qw_mx_gemv_kernel<QWHIP_BF16, false>);
     if (lds > 65536u) QWHIP_TRY_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));

@@ -302,7 +302,7 @@ def test_gemv(dev, m, n, k, ld, t):
 
 
 @pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
-@pytest.mark.parametrize("m,n,k", [(1, 40007, 64), (4, 17001, 544), (7, 9000, 2592), (16, 4500, 1056), (3, 5000, 3616), (2, 35, 33312), (1, 20, 90112)])
+@pytest.mark.parametrize("m,n,k", [(1, 40007, 64), (4, 17001, 544), (7, 9000, 2592), (16, 4500, 1056), (3, 5000, 3616), (2, 35, 33312), (1, 20, 90112), (9, 333, 17408), (11, 2116, 8768), (16, 4200, 8224)])
 def test_gemv_workgroups_with_several_tiles_and_long_rows(dev, t, m, n, k):
     bank = random_bank(n, k, n)
     wv, bufs = put_bank(dev, bank, k)
