@@ -405,3 +405,67 @@ def test_gemv_captured(dev):
         assert np.array_equal(y.download(np.float32, (m, n)), want)
     g.destroy()
     free(xb, y, *bufs)
+
+
+@pytest.mark.parametrize("m,n,k", [(512, 640, 8192), (300, 4000, 640), (2048, 5100, 288)])
+def test_gemm_forms_captured(dev, m, n, k):
+    """The tiled kernel, with K ranges where there is room for them, recorded and replayed: the eager bits."""
+    wb, xb = random_bank(n, k, 1), random_bank(m, k, 2)
+    wv, b0 = put_bank(dev, wb, k)
+    xv, b1 = put_bank(dev, xb, k)
+    room = filled(dev, dev.lib.qwhip_mxfp4_gemm_workspace_bytes(m, n, k), 0x7FC00000)
+    want = gemm(dev, wv, xv, m, n, qwhip.F32, workspace=room)
+    y, st = dev.alloc(m * n * 4), qwhip.Stream(dev)
+    g = qwhip.Graph(st, lambda: qwhip.check(dev.lib.qwhip_mxfp4_gemm(st.handle, C.byref(wv), C.byref(xv), y.ptr, qwhip.F32, 0, room.ptr, room.nbytes)))
+    for _ in range(3):
+        qwhip.check(dev.lib.qwhip_fill_u32(dev.stream.handle, y.ptr, 0, m * n))
+        qwhip.check(dev.lib.qwhip_fill_u32(dev.stream.handle, room.ptr, 0x7FC00000, room.nbytes // 4))
+        dev.stream.sync()
+        g.launch()
+        st.sync()
+        assert np.array_equal(y.download(np.float32, (m, n)), want)
+    g.destroy()
+    check_product(want, xb[2], wb[2], qwhip.F32)
+    free(y, room, *b0, *b1)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 200, 17408), (13, 640, 12800), (2, 96, 17408)])
+def test_gemv_with_much_lds_captured(dev, m, n, k):
+    bank = random_bank(n, k, 6)
+    wv, bufs = put_bank(dev, bank, k)
+    image, val = as_type(np.random.default_rng(1).standard_normal((m, k)), qwhip.BF16)
+    xb, y, st = dev.put(image), dev.alloc(m * n * 4), qwhip.Stream(dev)
+    g = qwhip.Graph(st, lambda: qwhip.check(dev.lib.qwhip_mxfp4_gemv(st.handle, C.byref(wv), xb.ptr, qwhip.BF16, m, None, y.ptr)))
+    _, want = gemv(dev, wv, image, qwhip.BF16, m, n)
+    for _ in range(3):
+        qwhip.check(dev.lib.qwhip_fill_u32(dev.stream.handle, y.ptr, 0, m * n))
+        dev.stream.sync()
+        g.launch()
+        st.sync()
+        assert np.array_equal(y.download(np.float32, (m, n)), want)
+    g.destroy()
+    check_product(want, val.astype(np.float64), bank[2], qwhip.F32)
+    free(xb, y, *bufs)
+
+
+def test_quantise_and_dequant_captured(dev):
+    rows, k = 33, 1056
+    x = np.random.default_rng(7).standard_normal((rows, k)).astype(np.float32)
+    src, codes, scales, values, out = dev.put(x), dev.alloc(rows * k // 2), dev.alloc(rows * k // 32), dev.alloc(rows * k * 4), dev.alloc(rows * k * 4)
+    v, st = view(codes, scales, rows, k), qwhip.Stream(dev)
+
+    def both():
+        qwhip.check(dev.lib.qwhip_quantize_mxfp4(st.handle, src.ptr, qwhip.F32, rows, k, 0, codes.ptr, scales.ptr, values.ptr))
+        qwhip.check(dev.lib.qwhip_dequant_mxfp4(st.handle, C.byref(v), out.ptr, qwhip.F32))
+
+    g = qwhip.Graph(st, both)
+    for turn in range(3):
+        x = np.random.default_rng(turn).standard_normal((rows, k)).astype(np.float32)
+        src.upload(x)
+        g.launch()
+        st.sync()
+        want = qwmx.values(*qwmx.quantise(x))
+        assert np.array_equal(values.download(np.float32, (rows, k)).astype(np.float64), want)
+        assert np.array_equal(out.download(np.float32, (rows, k)).astype(np.float64), want)
+    g.destroy()
+    free(src, codes, scales, values, out)
