@@ -575,7 +575,7 @@ qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const
 uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
 /* Decode / verify: y [m, n] = x . W^T for m = 1..16 rows (0: nothing to do) of f16 or bf16 activations [m, k], tight and 16-byte
  * aligned, not quantised; y16 (f16) and / or y32 (f32), at least one.  Every weight byte is read once for all rows (twice for
- * nine and more long rows on few outputs); fp32 accumulation in an order that follows from m, n, k and, for f16, from the scales. */
+ * nine and more long rows on few outputs); fp32 accumulation in an order that follows from m, n, k and the scales. */
 qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_view* w, const void* x, uint32_t x_dtype, uint32_t m, void* y16,
                               float* y32);
 

@@ -39,16 +39,15 @@ __device__ __forceinline__ f4_t qw_mfma16(u4_t a, u4_t b, f4_t c) {
 // A workgroup keeps x in LDS (all of it, or chunk after chunk) and takes tiles of 16 weight rows, a tile's columns dealt to `ways` waves in
 // steps of 16 blocks (512 columns).  Lane (i, g) has blocks g, 4 + g, 8 + g, 12 + g of a step of weight row i and the step's 16 scales of
 // that row, a step ahead of their use.
-// bf16: the scaled elements are bf16 numbers, so a lane turns its block into four operands and the matrix unit contracts them with the
-// same columns of x.
-// f16: so they are for scales of 2^-13 .. 2^13, whose elements are normal f16 numbers; where a wave's step has all of its scales there, it is
-// taken the same way.  Other scales: the codes go in unscaled.  A transpose over the lane rows leaves a lane eight codes of each of four
-// blocks; a matrix instruction then contracts one block, and the block's scale multiplies its fp32 sums.  (A block's instructions: 22 the
+// The scaled elements are numbers of x's type where the scale is 2^-13 .. 2^13 (f16: normal numbers then) or at most 2^125 (bf16: 6 x 2^126 is
+// past its range).  Where a wave's step has all of its scales there, a lane turns its block into four operands and the matrix unit contracts
+// them with the same columns of x.  Otherwise the codes go in unscaled.  A transpose over the lane rows leaves a lane eight codes of each of
+// four blocks; a matrix instruction then contracts one block, and the block's scale multiplies its fp32 sums.  (A block's instructions: 22 the
 // first way, 54 the second.)
 // Bound by the weights' bytes on long banks (151936 x 5120, one row: 75 us = 5.5 TB/s, at the rate of a large copy), by start and end of the
 // launch on shorter ones (17408 x 5120: 12.1 us = 3.9 TB/s).  x straight from memory instead of LDS, four of its lines for one of weights,
 // took 14.7 and 114 us.  Eight f16 rows of 17408 columns pass x through LDS once for 32 weight rows: 17.6 us (19.3 with every step unscaled).
-constexpr uint32_t QW_MX_GEMV_STEP = 16, QW_MX_GEMV_AHEAD = 4, QW_MX_F16_LEAST = 114, QW_MX_F16_MOST = 140;
+constexpr uint32_t QW_MX_GEMV_STEP = 16, QW_MX_GEMV_AHEAD = 4, QW_MX_F16_LEAST = 114, QW_MX_F16_MOST = 140, QW_MX_BF16_MOST = 252;
 struct qw_mx_gemv_load {   // what a lane carries of a step of weights
     u4_t q[4], sc;
 };
@@ -81,14 +80,11 @@ __device__ __forceinline__ void qw_mx_gemv_multiply(const qw_mx_gemv_load& l, co
     uint32_t byte[4];
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) byte[u] = (l.sc[u] >> (8u * g)) & 0xFFu;
-    bool scaled = true;
-    if constexpr (DT == QWHIP_F16) {
-        uint32_t far = 0;
+    constexpr uint32_t LEAST = DT == QWHIP_F16 ? QW_MX_F16_LEAST : 0u, MOST = DT == QWHIP_F16 ? QW_MX_F16_MOST : QW_MX_BF16_MOST;
+    uint32_t far = 0;
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) far = max(far, byte[u] - QW_MX_F16_LEAST);
-        scaled = __ballot(far > QW_MX_F16_MOST - QW_MX_F16_LEAST) == 0ull;
-    }
-    if (scaled) {
+    for (uint32_t u = 0; u < 4; ++u) far = max(far, byte[u] - LEAST);
+    if (__ballot(far > MOST - LEAST) == 0ull) {
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             const float s = __uint_as_float(byte[u] << 23);
