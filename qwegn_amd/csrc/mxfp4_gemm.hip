@@ -409,6 +409,7 @@ static qw_mx_plan qw_mx_choose(uint32_t m, uint32_t n, uint32_t blocks, bool til
         const qw_mx_form& t = g_mx_forms[f];
         if (m < t.bm || n < t.bn) continue;
         const uint64_t tiles = (uint64_t)qwhip_cdiv(m, t.bm) * qwhip_cdiv(n, t.bn), plane = (uint64_t)m * qw_mx_pitch(n) * 4u;
+        if (tiles > (1u << 22)) continue;   // 2^31 threads
         for (uint32_t want = 1; want <= 16u; ++want) {
             const uint32_t range = (qwhip_cdiv(stages, want) + 1u) & ~1u, ranges = qwhip_cdiv(stages, range);   // whole steps of scales
             if (want > 1u && (ranges != want || ranges * plane > room || tiles * ranges > 512u)) continue;
@@ -446,7 +447,6 @@ extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_vie
     if (ldy < w->n) return qwhip_fail(QWHIP_E_BAD_SHAPE, "output row pitch %u is under n=%u", ldy, w->n);
     if ((uintptr_t)y & (y_dtype == QWHIP_F32 ? 3u : 1u)) return qwhip_fail(QWHIP_E_BAD_SHAPE, "GEMM output is not aligned to its elements");
     if ((uintptr_t)workspace & 15u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "GEMM workspace must be 16-byte aligned");
-    if (x->n > 65535u * 32u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows do not fit one launch", x->n);
     QW_ON_DEVICE_OF(s);
     const qw_mx_operand ow = {(const uint8_t*)w->codes, (const uint8_t*)w->scales, w->n, qw_mxfp4_ld(w) / 32u};
     const qw_mx_operand ox = {(const uint8_t*)x->codes, (const uint8_t*)x->scales, x->n, qw_mxfp4_ld(x) / 32u};
@@ -466,10 +466,19 @@ extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_vie
     } else if (plan.form != QW_MX_ROWS_FORM) {
         qw_mx_launch_form(s, plan.form, {ow, ox, y, blocks, ldy, 0, 0, plan.range}, 1, y_dtype);
     } else {
-        const dim3 grid(qwhip_cdiv(w->n, 32u), qwhip_cdiv(x->n, 32u)), block(64u * min(16u, qwhip_cdiv(blocks, 16u)));
-        if (y_dtype == QWHIP_F32) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F32>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
-        else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F16>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
-        else hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_BF16>, grid, block, 0, s->stream, ow, ox, blocks, y, ldy);
+        // slabs of rows that one launch's grid and threads hold: one in all but extreme calls
+        constexpr uint32_t SLAB_N = 1u << 26, SLAB_M = 65535u * 32u;
+        const dim3 block(64u * min(16u, qwhip_cdiv(blocks, 16u)));
+        for (uint64_t n0 = 0; n0 < w->n; n0 += SLAB_N)
+            for (uint64_t m0 = 0; m0 < x->n; m0 += SLAB_M) {
+                const qw_mx_operand sw = {ow.codes + n0 * ow.ld32 * 16u, ow.scales + n0 * ow.ld32, (uint32_t)min((uint64_t)SLAB_N, w->n - n0), ow.ld32};
+                const qw_mx_operand sx = {ox.codes + m0 * ox.ld32 * 16u, ox.scales + m0 * ox.ld32, (uint32_t)min((uint64_t)SLAB_M, x->n - m0), ox.ld32};
+                void* const sy = (uint8_t*)y + (m0 * ldy + n0) * (y_dtype == QWHIP_F32 ? 4u : 2u);
+                const dim3 grid(qwhip_cdiv(sw.rows, 32u), qwhip_cdiv(sx.rows, 32u));
+                if (y_dtype == QWHIP_F32) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F32>, grid, block, 0, s->stream, sw, sx, blocks, sy, ldy);
+                else if (y_dtype == QWHIP_F16) hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_F16>, grid, block, 0, s->stream, sw, sx, blocks, sy, ldy);
+                else hipLaunchKernelGGL(qw_mx_gemm_rows_kernel<QWHIP_BF16>, grid, block, 0, s->stream, sw, sx, blocks, sy, ldy);
+            }
     }
     QWHIP_TRY_HIP(hipGetLastError());
     return QWHIP_OK;

@@ -7,7 +7,7 @@ import pytest
 
 from oracle import qwmx
 from qwegn_amd import qwhip
-from tests.test_gpu_mxfp4 import as_type, check_product, free, gemv, put_bank, random_bank
+from tests.test_gpu_mxfp4 import as_type, check_product, free, gemm, gemv, put_bank, random_bank
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,16 @@ def test_gemv_nan_block_beside_scales_that_reach_past_bf16(dev):
     w[11:13] = 0.0
     check_product(np.where(nan, 0.0, y32), val.astype(np.float64), w, qwhip.F32)
     free(*bufs)
+
+
+@pytest.mark.parametrize("n,ldy,t", [(5, 7, qwhip.F32), (33, 0, qwhip.BF16), (130, 0, qwhip.BF16)])
+def test_gemm_of_millions_of_rows(dev, n, ldy, t):
+    """More rows than the second dimension of a grid has tiles of: every row is there, checked at both ends and about the seam."""
+    m, k = 65535 * 32 + 70, 32
+    wb, xb = random_bank(n, k, 1), random_bank(m, k, 2, ld=64)
+    wv, b0 = put_bank(dev, wb, k)
+    xv, b1 = put_bank(dev, xb, k)
+    got = gemm(dev, wv, xv, m, n, t, ldy=ldy)
+    for at in (0, m // 2, m - 600, m - 300):
+        check_product(got[at:at + 300], xb[2][at:at + 300], wb[2], t)
+    free(*b0, *b1)
