@@ -605,9 +605,9 @@ typedef struct qwhip_logits_rules {
 } qwhip_logits_rules;
 /* logits [rows, n] f32, f16 or bf16 with row pitch ld (0 = n) -> out (same type, row pitch ld_out; may be logits itself at the
  * same pitch; NULL: not written) and tokens i32 [rows] (NULL: not asked for): the largest of the row's fp32 results, before they
- * are rounded to out's type, by the key rule of qwhip_argmax_f32 (NaN never wins against a number, ties to the lower token); -1
- * where nothing is above -inf, as behind a mask that allows no token.  Tokens need a workspace (8-byte aligned) of
- * qwhip_logits_workspace_bytes(rows, n) bytes, which the call writes before it reads; two calls that overlap in time take two.
+ * are rounded to out's type, by the key rule of qwhip_argmax_f32 (NaN never wins against a number, +0 is above -0, ties to the
+ * lower token); -1 where nothing is above -inf, as behind a mask that allows no token.  Tokens need a workspace (8-byte aligned)
+ * of qwhip_logits_workspace_bytes(rows, n) bytes, which the call writes before it reads; two calls that overlap in time take two.
  * rows <= 65535 (0: nothing to do), n < 2^30. */
 qwhip_status qwhip_logits_process(qwhip_stream_t s, const qwhip_logits_rules* rules, const void* logits, uint32_t dtype,
                                   uint32_t rows, uint32_t n, uint32_t ld, void* out, uint32_t ld_out, int32_t* tokens,

@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import numpy as np
 
+from oracle import qworacle as qo
+
 GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 BORDERS = 0.5 * (GRID[1:] + GRID[:-1])
 SIGNED = np.concatenate([GRID, -GRID])
@@ -62,6 +64,5 @@ def logits_f32(l, hist=None, prompt=None, total=None, rep=None, pres=None, freq=
                 at = r if allowed_row is None else int(allowed_row[r])
                 if 0 <= at < len(allowed):
                     l[r] = np.where(allowed[at], l[r], -np.inf)
-            x = np.where(np.isnan(l[r]), -np.inf, l[r])
-            tokens[r] = -1 if not (x > -np.inf).any() else int(np.argmax(x))
+            tokens[r] = qo.head_argmax(l[r])[0] if (l[r] > -np.inf).any() else -1   # the key rule: +0 is above -0
     return l, tokens
