@@ -573,6 +573,9 @@ qwhip_status qwhip_dequant_mxfp4(qwhip_stream_t s, const qwhip_mxfp4_view* v, vo
 qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const qwhip_mxfp4_view* x, void* y, uint32_t y_dtype,
                               uint32_t ldy, void* workspace, uint64_t workspace_bytes);
 uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
+/* The kernel form that a call with this much room takes (pitches under 2^23 elements), for tuning and tests: 0 .. 3 = tiles of
+ * 256 x 256, 256 x 192, 128 x 128, 64 x 128, 4 = the kernel for few tiles; *ranges (may be NULL) = its K ranges. */
+uint32_t qwhip_mxfp4_gemm_form(uint32_t m, uint32_t n, uint32_t k, uint64_t workspace_bytes, uint32_t* ranges);
 /* Decode / verify: y [m, n] = x . W^T for m = 1..16 rows (0: nothing to do) of f16 or bf16 activations [m, k], tight and 16-byte
  * aligned, not quantised; y16 (f16) and / or y32 (f32), at least one.  Every weight byte is read once for all rows (twice for
  * nine and more long rows on few outputs); fp32 accumulation in an order that follows from m, n, k and the scales. */

@@ -423,6 +423,13 @@ static qw_mx_plan qw_mx_choose(uint32_t m, uint32_t n, uint32_t blocks, bool til
     return best;
 }
 
+extern "C" uint32_t qwhip_mxfp4_gemm_form(uint32_t m, uint32_t n, uint32_t k, uint64_t workspace_bytes, uint32_t* ranges) {
+    const bool some = m != 0 && n != 0 && k != 0 && k % 32u == 0;
+    const qw_mx_plan plan = some ? qw_mx_choose(m, n, k / 32u, true, workspace_bytes) : qw_mx_plan{QW_MX_ROWS_FORM, 1u, 0u};
+    if (ranges) *ranges = plan.ranges;
+    return plan.form;
+}
+
 extern "C" uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
     if (m == 0 || n == 0 || k == 0 || k % 32u != 0) return 0;
     const qw_mx_plan plan = qw_mx_choose(m, n, k / 32u, true, ~(uint64_t)0);

@@ -133,6 +133,7 @@ SIGNATURES = {
     "qwhip_dequant_mxfp4": (C.c_int32, [_P, C.POINTER(Mxfp4View), _P, _U32]),
     "qwhip_mxfp4_gemm": (C.c_int32, [_P, C.POINTER(Mxfp4View), C.POINTER(Mxfp4View), _P, _U32, _U32, _P, _U64]),
     "qwhip_mxfp4_gemm_workspace_bytes": (_U64, [_U32, _U32, _U32]),
+    "qwhip_mxfp4_gemm_form": (_U32, [_U32, _U32, _U32, _U64, C.POINTER(C.c_uint32)]),
     "qwhip_mxfp4_gemv": (C.c_int32, [_P, C.POINTER(Mxfp4View), _P, _U32, _U32, _P, _P]),
     "qwhip_logits_process": (C.c_int32, [_P, C.POINTER(LogitsRules), _P, _U32, _U32, _U32, _U32, _P, _U32, _P, _P, _U64]),
     "qwhip_logits_workspace_bytes": (_U64, [_U32, _U32]),
