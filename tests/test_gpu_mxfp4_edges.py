@@ -91,6 +91,29 @@ def exact_product(x, w, unit):
     return x @ w.T
 
 
+GEMV_EXACT = [(1, 20, 90112), (1, 37, 90240), (2, 35, 33312), (2, 500, 33280), (3, 70, 22048), (5, 333, 17408), (8, 96, 7712), (9, 333, 17440), (16, 4200, 8224), (13, 64, 4640),   # chunks
+              (1, 40007, 64), (4, 17001, 544), (7, 9000, 2592), (3, 5000, 3616), (1, 640, 5152), (16, 20, 4096), (11, 4500, 1056), (2, 3, 32), (6, 33, 480)]
+
+
+@pytest.mark.parametrize("t", [qwhip.F16, qwhip.BF16])
+@pytest.mark.parametrize("kind", ["near", "far", "mixed"])
+@pytest.mark.parametrize("m,n,k", GEMV_EXACT)
+def test_gemv_exact_sums(dev, t, kind, m, n, k):
+    """Scales that leave the elements numbers of x's type, scales that do not, both within steps."""
+    near, far, mixed = ([120, 121, 122], [100, 101, 102], [111, 114, 117]) if t == qwhip.F16 else ([120, 121, 122], [252, 253, 254], [249, 252, 254])
+    scale_bytes = dict(near=near, far=far, mixed=mixed)[kind]
+    down = 100 if scale_bytes[-1] > 200 else 0                  # so far down are x and, here, w's values instead of it
+    bank = exact_bank(n, k, n + k, scale_bytes)
+    x = np.random.default_rng(m).integers(-1, 2, (m, k)).astype(np.float32)
+    image, _ = as_type(x * np.float32(2.0 ** -down), t)
+    w = (qwmx.values(bank[0], bank[1]) * 2.0 ** -down).astype(np.float32)
+    want = exact_product(x, w, 0.5 * 2.0 ** (scale_bytes[0] - 127 - down))
+    wv, bufs = put_bank(dev, bank, k)
+    _, y32 = gemv(dev, wv, image, t, m, n)
+    assert np.array_equal(y32, want)
+    free(*bufs)
+
+
 def form_of(dev, m, n, k, room):
     r = C.c_uint32()
     return dev.lib.qwhip_mxfp4_gemm_form(m, n, k, room, C.byref(r)), r.value
