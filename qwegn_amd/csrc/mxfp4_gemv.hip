@@ -225,9 +225,10 @@ extern "C" qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_vie
     }
     const bool chunked = ways > 16u;
     if (chunked) {
-        // nine and more rows: four tiles a workgroup, unless that leaves most units idle: then two groups of rows, each with the weights
-        // (11 rows of 8768 on 2116 outputs, 34 workgroups of four tiles: 17.8 -> 12.2 us; 16 rows of 17408 on 5120, 80 of them: 32.3 -> 34.5)
-        if (m > 8u && qwhip_cdiv(tiles, 4u) < 64u) group = (m + 1u) / 2u;
+        // nine and more rows: four tiles a workgroup, unless two groups of rows, each with the weights and two tiles a workgroup, still run in
+        // one round of the units (9 rows of 8768 on up to 64 fours of tiles 17.9 -> 11.8 us, on 72 to 160 fours 17.9 .. 20.2 -> 20.8 ..
+        // 32.7; 16 rows of 17408: 29.7 -> 18.3, 34.1 .. 37.5 -> 33.7 .. 58.0)
+        if (m > 8u && qwhip_cdiv(tiles, 4u) <= 64u) group = (m + 1u) / 2u;
         row_tiles = group > 8u ? 4u : 2u, ways = 16u / row_tiles;
         chunk = ways, chunks = qwhip_cdiv(steps, chunk);
         lds = 2u * group * (chunk * 1024u + 16u) + 16u * 1024u;   // at most 144 KB

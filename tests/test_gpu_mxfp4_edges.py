@@ -91,7 +91,7 @@ def exact_product(x, w, unit):
     return x @ w.T
 
 
-GEMV_EXACT = [(1, 20, 90112), (1, 37, 90240), (2, 35, 33312), (2, 500, 33280), (3, 70, 22048), (5, 333, 17408), (8, 96, 7712), (9, 333, 17440), (16, 4200, 8224), (13, 64, 4640),   # chunks
+GEMV_EXACT = [(1, 20, 90112), (1, 37, 90240), (2, 35, 33312), (2, 500, 33280), (3, 70, 22048), (5, 333, 17408), (8, 96, 7712), (9, 333, 17440), (16, 4200, 8224), (13, 64, 4640), (9, 4096, 8768), (16, 4095, 8704), (12, 4097, 8736),   # chunks
               (1, 40007, 64), (4, 17001, 544), (7, 9000, 2592), (3, 5000, 3616), (1, 640, 5152), (16, 20, 4096), (11, 4500, 1056), (2, 3, 32), (6, 33, 480)]
 
 
