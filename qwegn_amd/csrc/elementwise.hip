@@ -616,12 +616,6 @@ extern "C" qwhip_status qwhip_rmsnorm(qwhip_stream_t s, const void* x_f16, const
 // never wins against a number), key lo = ~row, larger (hi, lo) wins: ties go to the lower row.
 // One workgroup per logits row; 16-byte loads, eight in flight per thread; wave fold by lane exchanges, then LDS across waves.
 // ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t qw_sortable_f32(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
-    return (u & 0x80000000u) ? ~u : (u ^ 0x80000000u);
-}
-
 // One workgroup's vector ALU and its loads in flight bound the fold, so the sweep keeps a float maximum and its first row
 // per thread (a strict "greater" per element; NaN is never greater) and builds the 64-bit keys only to combine the 1024
 // thread results.  That is exact unless the row's maximum is a zero (+0.0 beats -0.0 in the key order, they are equal as

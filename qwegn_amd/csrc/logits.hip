@@ -22,12 +22,6 @@ struct qw_logits_args {
     uint32_t n, ld, ld_out, parts;
 };
 
-// The bits of a float made monotone; NaN is below everything but a hole (key 0).
-__device__ __forceinline__ uint32_t qw_lg_sortable(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
-    return (u & 0x80000000u) ? ~u : (u ^ 0x80000000u);
-}
 // A key's token; -1 where nothing is above -inf (whose key is 0x007FFFFF).
 __device__ __forceinline__ int32_t qw_lg_token(unsigned long long key) { return (uint32_t)(key >> 32) <= 0x007FFFFFu ? -1 : (int32_t)~(uint32_t)key; }
 
@@ -98,7 +92,7 @@ __global__ __launch_bounds__(QW_LG_THREADS) void qw_logits_kernel(const qw_logit
         const uint32_t i = tid + e * QW_LG_THREADS, tok = lo + i;
         if (i < len) {
             if (((allowed[e] >> (tok & 31u)) & 1u) == 0u) l[e] = -__builtin_inff();
-            const uint32_t k = qw_lg_sortable(l[e]);
+            const uint32_t k = qw_sortable_f32(l[e]);
             if (k > key) key = k, at = tok;
             if (a.out) {
                 const uint64_t o = (uint64_t)row * a.ld_out + tok;

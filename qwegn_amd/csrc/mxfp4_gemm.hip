@@ -8,8 +8,6 @@
 // bytes of block g of row i and its scale byte, which are a block as the container stores it.  D: lane (i, g) has rows 4 g .. 4 g + 3 of
 // the first operand in column i of the second.  Taken with W first, so that a lane holds four consecutive columns of Y.
 // ------------------------------------------------------------------------------------------------
-typedef __bf16 qw_bf4_t __attribute__((ext_vector_type(4)));
-
 struct qw_mx_operand {
     const uint8_t* codes;
     const uint8_t* scales;
@@ -439,7 +437,6 @@ extern "C" uint64_t qwhip_mxfp4_gemm_workspace_bytes(uint32_t m, uint32_t n, uin
 extern "C" qwhip_status qwhip_mxfp4_gemm(qwhip_stream_t s, const qwhip_mxfp4_view* w, const qwhip_mxfp4_view* x, void* y, uint32_t y_dtype, uint32_t ldy,
                                          void* workspace, uint64_t workspace_bytes) {
     QWHIP_REQUIRE(s);
-    (void)workspace, (void)workspace_bytes;
     qwhip_status st = qwhip_mxfp4_view_validate(w);
     if (st != QWHIP_OK) return st;
     QWHIP_REQUIRE(x);

@@ -102,6 +102,14 @@ __device__ __forceinline__ uint16_t qw_f32_to_bf16(float f) {
     return (uint16_t)(u >> 16);
 }
 
+// The bits of a float made monotone as an unsigned integer; NaN is 0, below every number (qw_sortable_f32_u32,
+// Sources/QWMetal/include/qw_fastmath_safe.metalh:21-25).
+__device__ __forceinline__ uint32_t qw_sortable_f32(float x) {
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+    return (u & 0x80000000u) ? ~u : (u ^ 0x80000000u);
+}
+
 // Load element i of a typed activation array as fp32.
 template <int DT>
 __device__ __forceinline__ float qw_load_f32(const void* p, uint64_t i) {
