@@ -24,19 +24,20 @@ extern "C" qwhip_status qwhip_mxfp4_view_validate(const qwhip_mxfp4_view* v) {
 //
 // Four neighbouring lanes share a block, eight elements each: whole lines per load and store, the maximum by two exchanges inside the
 // quad (as integers: magnitudes order like their bits, and infinities and NaN stay on top).  Bound by its bytes: 17408 x 5120 bf16 with
-// the values, 404 MB: 65.5 us = 6.2 TB/s, over what a large copy reaches; one row of 5120: 1.4 us on the device.
+// the values, 404 MB, more than half of them written: 64 us = 6.3 TB/s (a copy of 4 GiB 4.7 .. 5.0, a fill 6.9); one row of 5120: 1.4 us on
+// the device.
 // ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t qw_quad_umax(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
 }
 
-// Eight values, streamed past the caches (17408 x 5120 bf16 with values: 67.2 -> 65.5 us).
+// Eight values: 16-bit ones streamed past the caches (17408 x 5120 bf16 with values: 67.2 -> 65.5 us); a lane's 32 bytes of fp32 are two stores of
+// half lines, which wait in the L2 for each other (dequant of 17408 x 5120: 138 us streamed, 78 this way; quantised with values 135 -> 134).
 template <int DT>
 __device__ __forceinline__ void qw_stream8(void* dst, uint64_t at, const float* f) {
     if constexpr (DT == QWHIP_F32) {
-        __builtin_nontemporal_store(f4_t{f[0], f[1], f[2], f[3]}, (f4_t*)((float*)dst + at));
-        __builtin_nontemporal_store(f4_t{f[4], f[5], f[6], f[7]}, (f4_t*)((float*)dst + at + 4));
+        qw_store8_f32((float*)dst + at, f);
     } else if constexpr (DT == QWHIP_F16) {
         h8_t o;
 #pragma unroll
@@ -135,7 +136,9 @@ extern "C" qwhip_status qwhip_quantize_mxfp4(qwhip_stream_t s, const void* src, 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Reader: the values of a bank, [n, k] row-major.  Exact in bf16 and fp32; f16 rounds what its range does not hold.
+// Reader: the values of a bank, [n, k] row-major.  Exact in bf16 and fp32; f16 rounds what its range does not hold.  A lane has eight elements of
+// a quarter of a block: whole lines per load and store.  Bound by its bytes: 17408 x 5120 to f16 or bf16, 226 MB, 31.7 us = 7.1 TB/s, mostly
+// writes; to fp32, 404 MB, 78 us = 5.2 TB/s.
 // ------------------------------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(256) void qw_dequant_mxfp4_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ out,
