@@ -6,8 +6,9 @@
 // through the row's history (a few kB that stay in the L2) and counts in LDS the tokens that fall into its slice: the low bits of a word how
 // often in the answer, the top bit whether at all.  Integer additions commute: the counts do not depend on the order.  Where the row has
 // biases the same words then hold the largest index + 1 of a token's entries: of two entries for a token the later one holds.
-// Bound by the logits' bytes for a full batch: 256 rows of 151936 fp32, history 2048, 64 masks: 73 us = 4.3 TB/s (82 with cached stores);
-// by latency for one row (history 4096): 7.3 us with the token's launch.  More tokens a thread pay for a workgroup's chain of loads and the
+// Bound by the logits' bytes for a full batch: 256 rows of 151936 fp32, history 2048, 64 masks: 71 us = 4.4 TB/s (82 with cached stores); by
+// the work on a token for 16-bit logits, half the bytes in 57 us (a 2-byte load and store a lane); by latency for one row (history 4096):
+// 7.3 us with the token's launch.  More tokens a thread pay for a workgroup's chain of loads and the
 // history's reading less often (the batch with 1 / 2 / 4 / 8 / 16: 259 / 186 / 124 / 77 / 73 us), fewer leave the row's slices on more
 // compute units (one row: 7.3 / 7.6 / 8.1 / 8.8 / 11.5).
 // ------------------------------------------------------------------------------------------------

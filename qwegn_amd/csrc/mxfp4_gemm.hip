@@ -93,8 +93,10 @@ __global__ __launch_bounds__(1024) void qw_mx_gemm_rows_kernel(qw_mx_operand w, 
 // place c ^ ((r >> 1) & 7), so that the 16 rows that a fragment read touches lie on all banks.  Scales come in steps of two stages, 16
 // bytes of a row: the scales of four fragments' rows in one block column form one word (the matrix instruction picks the byte), transposed
 // inside lane quads on their way into LDS.
-// 4096 x 17408 x 5120 on 256 x 256 tiles: 193 us = 3.8 PFLOP/s, the matrix unit busy 48 % of the cycles at the 1.77 GHz that the card holds
-// under it (17.3 cycles an instruction, 7.9 PFLOP/s, where nothing else runs); without the stores 179, without the loads into LDS 153.
+// 4096 x 17408 x 5120 on 256 x 256 tiles: 190 .. 194 us by card = 3.8 PFLOP/s, the matrix unit busy 48 % of the cycles at the 1.77 GHz that it
+// holds under this load (17.3 cycles an instruction, 7.9 PFLOP/s, where nothing else runs), LDS 27 %: a stage's fragments and scales are 204 KB,
+// 1170 cycles by the counter, against 2048 of matrix instructions on each of the four SIMDs.  Without the stores 179, without the loads into
+// LDS 153.
 // ------------------------------------------------------------------------------------------------
 template <int N, int I = 0, class F>
 __device__ __forceinline__ void qw_static_for(F&& f) {

@@ -44,9 +44,10 @@ __device__ __forceinline__ f4_t qw_mfma16(u4_t a, u4_t b, f4_t c) {
 // them with the same columns of x.  Otherwise the codes go in unscaled.  A transpose over the lane rows leaves a lane eight codes of each of
 // four blocks; a matrix instruction then contracts one block, and the block's scale multiplies its fp32 sums.  (A block's instructions: 22 the
 // first way, 54 the second.)
-// Bound by the weights' bytes on long banks (151936 x 5120, one row: 75 us = 5.5 TB/s, at the rate of a large copy), by start and end of the
-// launch on shorter ones (17408 x 5120: 12.1 us = 3.9 TB/s).  x straight from memory instead of LDS, four of its lines for one of weights,
-// took 14.7 and 114 us.  Eight f16 rows of 17408 columns pass x through LDS once for 32 weight rows: 17.6 us (19.3 with every step unscaled).
+// Bound by the weights' bytes on long banks (151936 x 5120, one row: 74 .. 75 us = 5.5 TB/s; eight times the rows, 3.3 GB that no cache holds,
+// 568 us = 5.8 TB/s), by start and end of the launch on shorter ones (17408 x 5120: 13.0 us = 3.6 TB/s from memory, 11.3 where the last-level
+// cache has the bank).  x straight from memory instead of LDS, four of its lines for one of weights, took 14.7 and 114 us.  Eight f16 rows of
+// 17408 columns pass x through LDS once for 32 weight rows: 21.2 us from memory, 17.5 from the cache (19.3 with every step unscaled).
 constexpr uint32_t QW_MX_GEMV_STEP = 16, QW_MX_GEMV_AHEAD = 4, QW_MX_F16_LEAST = 114, QW_MX_F16_MOST = 140, QW_MX_BF16_MOST = 252;
 struct qw_mx_gemv_load {   // what a lane carries of a step of weights
     u4_t q[4], sc;
@@ -214,8 +215,8 @@ extern "C" qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_vie
     QW_ON_DEVICE_OF(s);
     const uint32_t blocks = w->k / 32u, tiles = qwhip_cdiv(w->n, 16u), steps = qwhip_cdiv(blocks, QW_MX_GEMV_STEP);
     // 16 waves a compute unit carry what its memory pipe needs in flight: in four workgroups where four copies of x and of the sums fit its
-    // LDS, in two, in one (rows of 5120, 17408 outputs, one row: 12.1 / 12.5 / 13.5 us with 4 / 8 / 16 ways; 17408 -> 5120: 14.6 / 14.1 / 15.2;
-    // eight rows of 5120: 39.4 / 16.3 / 16.3).  Past that x passes through LDS in chunks of a step a way, the next one carried in registers.
+    // LDS, in two, in one (banks in the last-level cache, rows of 5120, 17408 outputs, one row: 12.1 / 12.5 / 13.5 us with 4 / 8 / 16 ways;
+    // 17408 -> 5120: 14.6 / 14.1 / 15.2; eight rows of 5120: 39.4 / 16.3 / 16.3).  Past that x passes through LDS in chunks of a step a way, the next one carried in registers.
     const uint64_t row = (uint64_t)steps * 1024u + 16u, lds_bytes = 160u << 10;
     uint64_t lds = 0;
     uint32_t row_tiles = 1, ways = 4, chunk = steps, chunks = 1, group = m;
@@ -226,8 +227,8 @@ extern "C" qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_vie
     const bool chunked = ways > 16u;
     if (chunked) {
         // nine and more rows: four tiles a workgroup, unless two groups of rows, each with the weights and two tiles a workgroup, still run in
-        // one round of the units (9 rows of 8768 on up to 64 fours of tiles 17.9 -> 11.8 us, on 72 to 160 fours 17.9 .. 20.2 -> 20.8 ..
-        // 32.7; 16 rows of 17408: 29.7 -> 18.3, 34.1 .. 37.5 -> 33.7 .. 58.0)
+        // one round of the units (banks in the last-level cache; 9 rows of 8768: 17.9 -> 11.8 us on 20 to 64 fours of tiles, 17.9 .. 20.2 ->
+        // 20.8 .. 32.7 on 72 to 160; 16 rows of 17408: 29.7 -> 18.3, then 34.1 .. 37.5 -> 33.7 .. 58.0)
         if (m > 8u && qwhip_cdiv(tiles, 4u) <= 64u) group = (m + 1u) / 2u;
         row_tiles = group > 8u ? 4u : 2u, ways = 16u / row_tiles;
         chunk = ways, chunks = qwhip_cdiv(steps, chunk);
