@@ -582,6 +582,104 @@ uint32_t qwhip_mxfp4_gemm_form(uint32_t m, uint32_t n, uint32_t k, uint64_t work
 qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_view* w, const void* x, uint32_t x_dtype, uint32_t m, void* y16,
                               float* y32);
 
+/* ---- between the q|k|v projection and the output projection ----------------------------------- */
+/* The reference has these steps outside of the path that this library rebuilds; the doors stand beside the norm, the MXFP4
+ * quantiser and the MXFP4 products, and use their conventions: they check before they enqueue, allocate nothing, keep nothing
+ * between calls and only launch kernels (a call can be captured); no door uses the stream's scratch. */
+
+/* What a layer does to its heads, in this order, in fp32, every operation rounded by itself:
+ *   norm      x_i = (x_i * r) * g_i, r = 1 / sqrt(mean(x^2) + eps) over the head; the squares are added as a tree (inside each eight
+ *             i and i + 4, then 2, then 1; the eights by halves, padded with zeros to a power of two)
+ *   rotation  the first rope_dims elements, a = x_i and b = x_{i + rope_dims / 2} (QWHIP_HEAD_ROPE_PAIRS: x_{2i} and x_{2i + 1}):
+ *             a c - b s, b c + a s with c, s of the row's position
+ *   FWHT-32   every 32 elements, as in qwhip_fwht32: queries and keys both (their product stays), values alone (the attention's
+ *             output is then in the basis of a rotated container: QWHIP_X_PREROTATED)
+ * A part whose pointer or flag is not set is left out. */
+enum {
+    QWHIP_HEAD_GAMMA_PLUS_ONE = 1u << 0, /* g = 1 + gamma, as in qwhip_rmsnorm; else g = gamma */
+    QWHIP_HEAD_ROPE_PAIRS = 1u << 1,     /* neighbouring elements turn together; else the halves of rope_dims */
+    QWHIP_HEAD_FWHT_QK = 1u << 2,
+    QWHIP_HEAD_FWHT_V = 1u << 3 /* qwhip_kv_append_mxfp4 */
+};
+typedef struct qwhip_head_rules {
+    const int32_t* position; /* [rows], required with cos_sin; a position outside the table takes the table's nearest row */
+    const float* cos_sin;    /* [positions, rope_dims], 16-byte aligned: rope_dims / 2 cosines, then the sines */
+    const void* q_gamma;     /* f16 [head_dim], 16-byte aligned; NULL: queries are not normed */
+    const void* k_gamma;     /* the same for keys */
+    uint32_t positions;      /* rows of the table */
+    uint32_t rope_dims;      /* a multiple of 16, at most head_dim */
+    float eps;
+    uint32_t flags;          /* QWHIP_HEAD_* */
+} qwhip_head_rules;
+/* Queries q [rows, q_heads, head_dim] with row pitch ld_q elements (0 = tight) and keys k [rows, k_heads, head_dim] with ld_k, f32,
+ * f16 or bf16, by the rules -> q_out, k_out in out_dtype (f32, f16 or bf16; pitches ld_q_out, ld_k_out).  Either side may be left
+ * out (no heads).  An output may be its own input (same type and pitch), otherwise outputs overlap no input.  head_dim a multiple of 32
+ * up to 256, rows 16-byte aligned; under 2^24 rows (0: nothing to do). */
+qwhip_status qwhip_head_norm_rope(qwhip_stream_t s, const qwhip_head_rules* rules, uint32_t rows, uint32_t head_dim, const void* q,
+                                  uint32_t q_heads, uint32_t ld_q, const void* k, uint32_t k_heads, uint32_t ld_k, uint32_t dtype,
+                                  void* q_out, uint32_t ld_q_out, void* k_out, uint32_t ld_k_out, uint32_t out_dtype);
+
+/* A paged cache of keys and values in MXFP4 (elements, blocks of 32 along the head, scale rule and NaN as in qwhip_quantize_mxfp4).
+ * pages: [page_count][kv_heads] pieces of page_size * head_dim * 17 / 16 bytes; a piece holds, with T tokens and D = head_dim,
+ *   keys' codes     [T][D / 2] bytes, element 2 i in the low half of byte i
+ *   keys' scales    [T][D / 32] bytes
+ *   values' codes   [T / 8][D / 8][8] words of eight elements (lowest element in the lowest nibble), token t at [t / 8][..][t % 8]
+ *   values' scales  [T / 8][D / 32][8] bytes
+ * (the values' eight tokens side by side are what a lane of the matrix unit contracts).  Scale bytes over 252, which only a block
+ * that was not finite gets, read as NaN. */
+typedef struct qwhip_kv_cache {
+    void* pages;         /* device, 16-byte aligned */
+    uint64_t bytes;      /* what the caller's region holds from there on */
+    uint32_t page_count; /* page_count * page_size < 2^31 */
+    uint32_t page_size;  /* tokens: 16, 32, 64, 128 or 256 */
+    uint32_t kv_heads;   /* 1 .. 1024 */
+    uint32_t head_dim;   /* 64, 128 or 256 */
+} qwhip_kv_cache;
+/* Bytes of one page over all heads; 0 for a geometry that is not taken. */
+uint64_t qwhip_kv_page_bytes(uint32_t page_size, uint32_t kv_heads, uint32_t head_dim);
+/* QWHIP_OK, QWHIP_E_BAD_WEIGHTS (geometry, size, alignment) or QWHIP_E_NULL. */
+qwhip_status qwhip_kv_cache_validate(const qwhip_kv_cache* c);
+/* A step's or a prompt's keys k and values v [rows, kv_heads, head_dim] (pitches ld_k, ld_v elements, 0 = tight; f32, f16 or bf16)
+ * into the cache: row r goes to token slots[r] % page_size of page slots[r] / page_size.  A row whose slot is negative or behind
+ * the cache is left out: nothing is written for it.  The slots of a call differ (what a slot holds that two rows name is not
+ * defined).  `rules` (NULL: none) apply to the keys on the way, QWHIP_HEAD_FWHT_V to the values, and to the queries q [rows, q_heads, head_dim]
+ * of the same rows, which the launch takes along into q_out (0 heads: none), as qwhip_head_norm_rope would, the same bits.
+ * k_values, v_values (each may be NULL): what the cache holds for the rows, [rows, kv_heads, head_dim] tight.  q_out and the values
+ * are in out_dtype; exact in f32 and bf16 as qwhip_dequant_mxfp4.  All rows 16-byte aligned; outputs overlap no input (q_out may be q,
+ * same type and pitch); under 2^24 rows. */
+qwhip_status qwhip_kv_append_mxfp4(qwhip_stream_t s, const qwhip_kv_cache* cache, const qwhip_head_rules* rules, uint32_t rows,
+                                   const int32_t* slots, const void* k, uint32_t ld_k, const void* v, uint32_t ld_v, uint32_t dtype,
+                                   const void* q, uint32_t q_heads, uint32_t ld_q, void* q_out, uint32_t ld_q_out, uint32_t out_dtype,
+                                   void* k_values, void* v_values);
+
+/* A batch's sequences.  Sequence i has the rows row_start[i] .. row_start[i + 1] - 1 of q and lengths[i] cached tokens, its own rows'
+ * among them: row j of n is at position lengths[i] - n + j.  Token t of a sequence is token t % page_size of page
+ * block_table[i][t / page_size].  All pointers are device memory; the bounds are the host's. */
+typedef struct qwhip_kv_batch {
+    const int32_t* row_start;   /* [seqs + 1], ascending; NULL: row i is sequence i's only one */
+    const int32_t* lengths;     /* [seqs] (what passes max_length is cut off) */
+    const int32_t* block_table; /* [seqs, ld_table]; an entry outside the cache is read as page 0 */
+    uint32_t ld_table;
+    uint32_t seqs;              /* up to 65535 */
+    uint32_t max_rows;          /* the most rows of a sequence: what passes it is left as it was */
+    uint32_t max_length;        /* the most tokens of a sequence, at most ld_table * page_size */
+} qwhip_kv_batch;
+/* out [rows, q_heads, head_dim] = softmax(scale q . K^T) V over the tokens at or before a row's position, and behind position - window
+ * with a window (0: none).  q and out f16 or bf16 (pitches ld_q, ld_out elements, 0 = tight; rows 16-byte aligned), query head h with
+ * key head h / (q_heads / kv_heads); q_heads <= 65535; scale > 0.  lse (may be NULL): f32 [rows, q_heads], the logarithm of the
+ * sum.  A row that sees no token, or only scores of -inf, gets zeros and lse = -inf; rows behind the last sequence's are left as they
+ * were.  A token that a row does not see does not reach it, whatever its page holds (NaN among it).
+ * fp32 softmax and sums of exact products with q; a weight is rounded to f16 in front of the product with the values.  Out overlaps
+ * neither q nor the cache.
+ * workspace (may be NULL; 16-byte aligned): lets few rows over long sequences split these over more compute units, partial results
+ * are joined in a fixed order; at most qwhip_kv_attention_workspace_bytes(..) bytes are used, less room gives fewer parts.  The parts follow
+ * from the shapes, the bounds and the room, so a row's bits may depend on them.  Two calls that overlap in time take two workspaces. */
+qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_kv_cache* cache, const qwhip_kv_batch* batch, const void* q,
+                                      uint32_t dtype, uint32_t q_heads, uint32_t ld_q, uint32_t rows, float scale, uint32_t window,
+                                      void* out, uint32_t ld_out, float* lse, void* workspace, uint64_t workspace_bytes);
+uint64_t qwhip_kv_attention_workspace_bytes(const qwhip_kv_cache* cache, const qwhip_kv_batch* batch, uint32_t q_heads, uint32_t rows,
+                                            uint32_t window);
+
 /* ---- from logits to the token ------------------------------------------------------ */
 /* What a step of a batch applies to its logits before a token is chosen, in this order, in fp32:
  *   seen in the row's history (prompt or answer): l = l > 0 ? l / repetition : l * repetition

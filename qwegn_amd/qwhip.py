@@ -19,6 +19,7 @@ KIND_HQ4_G32_M5, KIND_ROTATED_HQ, KIND_NATIVE_AFFINE = 0, 1, 2
 X_PREROTATED = 1
 GEMV_ROW_INVARIANT = 2
 MOE_REUSE_EXPERTS = 4
+HEAD_GAMMA_PLUS_ONE, HEAD_ROPE_PAIRS, HEAD_FWHT_QK, HEAD_FWHT_V = 1, 2, 4, 8
 
 
 class QwhipError(RuntimeError):
@@ -48,6 +49,21 @@ class LogitsRules(C.Structure):
     _fields_ = [(name, C.c_void_p) for name in ("history", "prompt_len", "total_len", "repetition", "presence", "frequency", "bias_off", "bias_tok",
                                                 "bias_val", "allowed", "allowed_row")]
     _fields_ += [(name, C.c_uint32) for name in ("ld_history", "bias_count", "allowed_rows", "ld_allowed")]
+
+
+class HeadRules(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("position", "cos_sin", "q_gamma", "k_gamma")]
+    _fields_ += [("positions", C.c_uint32), ("rope_dims", C.c_uint32), ("eps", C.c_float), ("flags", C.c_uint32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("bytes", C.c_uint64)]
+    _fields_ += [(name, C.c_uint32) for name in ("page_count", "page_size", "kv_heads", "head_dim")]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("row_start", "lengths", "block_table")]
+    _fields_ += [(name, C.c_uint32) for name in ("ld_table", "seqs", "max_rows", "max_length")]
 
 
 _P = C.c_void_p
@@ -135,6 +151,12 @@ SIGNATURES = {
     "qwhip_mxfp4_gemm_workspace_bytes": (_U64, [_U32, _U32, _U32]),
     "qwhip_mxfp4_gemm_form": (_U32, [_U32, _U32, _U32, _U64, C.POINTER(C.c_uint32)]),
     "qwhip_mxfp4_gemv": (C.c_int32, [_P, C.POINTER(Mxfp4View), _P, _U32, _U32, _P, _P]),
+    "qwhip_head_norm_rope": (C.c_int32, [_P, C.POINTER(HeadRules), _U32, _U32, _P, _U32, _U32, _P, _U32, _U32, _U32, _P, _U32, _P, _U32, _U32]),
+    "qwhip_kv_page_bytes": (_U64, [_U32, _U32, _U32]),
+    "qwhip_kv_cache_validate": (C.c_int32, [C.POINTER(KvCache)]),
+    "qwhip_kv_append_mxfp4": (C.c_int32, [_P, C.POINTER(KvCache), C.POINTER(HeadRules), _U32, _P, _P, _U32, _P, _U32, _U32, _P, _U32, _U32, _P, _U32, _U32, _P, _P]),
+    "qwhip_kv_attention_mxfp4": (C.c_int32, [_P, C.POINTER(KvCache), C.POINTER(KvBatch), _P, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _U32, _P, _P, _U64]),
+    "qwhip_kv_attention_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(KvBatch), _U32, _U32, _U32]),
     "qwhip_logits_process": (C.c_int32, [_P, C.POINTER(LogitsRules), _P, _U32, _U32, _U32, _U32, _P, _U32, _P, _P, _U64]),
     "qwhip_logits_workspace_bytes": (_U64, [_U32, _U32]),
     "qwhip_repack_mlx_affine": (C.c_int32, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
