@@ -1,5 +1,6 @@
 // Attention over the paged MXFP4 cache.
 #include "qw_kv.h"
+#include <stdlib.h>
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
@@ -30,6 +31,32 @@ __device__ __forceinline__ qw_attn_seq qw_attn_sequence(const qw_attn_args& a, u
     return s;
 }
 
+// The tokens that the columns c0 .. c1 of a sequence see together, from a step's border on, and this part's share of the steps.
+struct qw_attn_range {
+    int32_t pos_a, pos_b;        // positions of the first and the last column's rows; negative: sees nothing
+    uint32_t low_a, low_b;       // the first tokens that these see
+    uint32_t first, from, to;    // first token of the steps, this part's steps
+};
+__device__ __forceinline__ uint32_t qw_attn_low(const qw_attn_args& a, int32_t pos) {
+    return a.window && pos + 1 > (int32_t)a.window ? (uint32_t)(pos + 1 - (int32_t)a.window) : 0u;
+}
+template <uint32_t T>
+__device__ __forceinline__ qw_attn_range qw_attn_tokens(const qw_attn_args& a, const qw_attn_seq& s, uint32_t c0, uint32_t c1, uint32_t part) {
+    qw_attn_range r;
+    r.pos_a = (int32_t)(s.length - s.n + c0 / a.shared), r.pos_b = (int32_t)(s.length - s.n + c1 / a.shared);
+    r.low_a = qw_attn_low(a, r.pos_a), r.low_b = qw_attn_low(a, r.pos_b);
+    r.first = r.low_a & ~(T - 1u);
+    const uint32_t end = r.pos_b < 0 ? r.first : (uint32_t)r.pos_b + 1u;   // pos_b < 0: low_a is 0
+    const uint32_t steps = (end - r.first + T - 1u) / T, each = (steps + a.parts - 1u) / a.parts;
+    r.from = min(part * each, steps), r.to = min(r.from + each, steps);
+    return r;
+}
+// Scale bytes of eight tokens from `t` on, of which the ones behind the last are not there: a harmless one in their place.
+__device__ __forceinline__ u2_t qw_attn_tail(u2_t scales, uint32_t t, uint32_t length) {
+    const uint32_t n = length - t, lo = n >= 4u ? ~0u : (1u << (8u * n)) - 1u, hi = n >= 8u ? ~0u : n > 4u ? (1u << (8u * n - 32u)) - 1u : 0u;
+    return u2_t{(scales[0] & lo) | (0x7F7F7F7Fu & ~lo), (scales[1] & hi) | (0x7F7F7F7Fu & ~hi)};
+}
+
 // What a lane carries of a step of 32 tokens.  Keys: rows of two 16-row operands, lane (i, g) has elements of token 8 (i / 4) + 4 a + i % 4; values: lane
 // (i, g) has eight elements of each of the tokens 8 g .. 8 g + 7.  A score of operand a, accumulator row 4 g + r, is then token 8 g + 4 a + r: the weights
 // are in place as an operand against the values.
@@ -42,21 +69,21 @@ struct qw_attn_step {
     u2_t v_scale[SETS];
 };
 template <int D>
-__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride_lo, const int32_t* table, uint32_t first_page, uint32_t t0,
+__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t first_page, uint32_t t0,
                                              uint32_t length, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS;
     const uint32_t inside = (1u << a.geo.page_log2) - 1u, last = length - 1u;
-    // a group of eight tokens behind the last one's is read in its place, and masked
+    // of a group of eight tokens behind the last one's the last one's is read, and masked
     const uint32_t kt = min(t0 + 8u * (i >> 2), last & ~7u) + (i & 3u), vt = min(t0 + 8u * g, last & ~7u);
-    const uint8_t* const kp = head + (uint64_t)(uint32_t)table[(kt >> a.geo.page_log2) - first_page] * stride_lo;
-    const uint8_t* const vp = head + (uint64_t)(uint32_t)table[(vt >> a.geo.page_log2) - first_page] * stride_lo;
+    const uint8_t* const kp = head + (uint64_t)(uint32_t)table[(kt >> a.geo.page_log2) - first_page] * stride;
+    const uint8_t* const vp = head + (uint64_t)(uint32_t)table[(vt >> a.geo.page_log2) - first_page] * stride;
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
         const uint32_t t = (kt & inside) + 4u * h;
 #pragma unroll
         for (uint32_t c = 0; c < SETS; ++c) {
             __builtin_memcpy(s.k[h][c], __builtin_assume_aligned(kp + t * (D / 2u) + c * 64u + g * (4u * WORDS), 4 * WORDS), 4 * WORDS);
-            s.k_scale[h][c] = kp[a.geo.k_scales + t * (D / 32u) + (D == 64 ? g >> 1 : 4u * c + g)];
+            s.k_scale[h][c] = kt + 4u * h > last ? 127u : kp[a.geo.k_scales + t * (D / 32u) + (D == 64 ? g >> 1 : 4u * c + g)];
         }
     }
     const uint32_t t8 = (vt & inside) >> 3, word = D == 64 ? i & 7u : i;
@@ -65,7 +92,7 @@ __device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_
         const uint8_t* const w = vp + a.geo.v_codes + (t8 * (D / 8u) + 16u * c + word) * 32u;
         s.v[c][0] = *(const u4_t*)w;
         s.v[c][1] = *(const u4_t*)(w + 16);
-        s.v_scale[c] = *(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + 4u * c + (word >> 2)) * 8u);
+        s.v_scale[c] = qw_attn_tail(*(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + 4u * c + (word >> 2)) * 8u), vt, length);
     }
 }
 
@@ -87,6 +114,11 @@ __device__ __forceinline__ u4_t qw_attn_operand(uint32_t w, float scale) {
     return o;
 }
 template <int DT>
+__device__ __forceinline__ uint32_t qw_attn_pair(uint32_t w, float scale) {   // the two lowest
+    if constexpr (DT == QWHIP_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+}
+template <int DT>
 __device__ __forceinline__ f4_t qw_attn_mfma(u4_t a, u4_t b, f4_t c) {
     if constexpr (DT == QWHIP_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
@@ -94,276 +126,484 @@ __device__ __forceinline__ f4_t qw_attn_mfma(u4_t a, u4_t b, f4_t c) {
 // Two floats as bf16, the first in the low half.
 __device__ __forceinline__ uint32_t qw_attn_bf16x2(float a, float b) { return (uint32_t)qw_f32_to_bf16(a) | ((uint32_t)qw_f32_to_bf16(b) << 16); }
 
-// f16 holds the elements under a scale byte exactly, as normal numbers, from 2^-13 to 2^13; bf16 up to 2^125.
+// Eight f16 numbers as two bf16 numbers each, whose sum they are: eight bits and the last three (an infinity's or a NaN's rest is zero).
+__device__ __forceinline__ void qw_attn_split(u4_t q, u4_t& hi, u4_t& lo) {
+    const h8_t x = __builtin_bit_cast(h8_t, q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float x0 = (float)x[2 * e], x1 = (float)x[2 * e + 1];
+        const uint32_t h0 = __float_as_uint(x0) & 0xFFFF0000u, h1 = __float_as_uint(x1) & 0xFFFF0000u;
+        const float l0 = (h0 & 0x7F800000u) == 0x7F800000u ? 0.0f : x0 - __uint_as_float(h0), l1 = (h1 & 0x7F800000u) == 0x7F800000u ? 0.0f : x1 - __uint_as_float(h1);
+        hi[e] = (h0 >> 16) | h1;
+        lo[e] = (__float_as_uint(l0) >> 16) | (__float_as_uint(l1) & 0xFFFF0000u);
+    }
+}
+// Floats of an output row: 1, 2, 4 or 8.
+template <int DT, uint32_t E>
+__device__ __forceinline__ void qw_attn_store(uint16_t* y, const float* o) {
+    typedef uint16_t v_t __attribute__((ext_vector_type(E)));
+    v_t v;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) v[e] = DT == QWHIP_F16 ? __builtin_bit_cast(uint16_t, (h1_t)o[e]) : qw_f32_to_bf16(o[e]);
+    *(v_t*)y = v;
+}
+// f16 holds the elements under a scale byte as normal numbers, exactly, from 2^-13 to 2^13 (and the zeros of a block of zeros: byte 0, whose other elements are
+// under 2^-124 and count as zero); bf16 up to 2^125.
 constexpr uint32_t QW_ATTN_F16_LEAST = 114, QW_ATTN_F16_MOST = 140, QW_ATTN_BF16_MOST = 252;
+template <int DT>
+__device__ __forceinline__ bool qw_attn_far(uint32_t byte) {
+    return DT == QWHIP_F16 ? byte - QW_ATTN_F16_LEAST > QW_ATTN_F16_MOST - QW_ATTN_F16_LEAST && byte != 0u : byte > QW_ATTN_BF16_MOST;
+}
+__device__ __forceinline__ bool qw_attn_far8(u2_t scales) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) bad |= qw_attn_far<QWHIP_F16>((scales[e >> 2] >> (8u * (e & 3u))) & 0xFFu) ? 1u : 0u;
+    return bad != 0u;
+}
+__device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) { return __uint_as_float(((scales[e >> 2] >> (8u * (e & 3u))) & 0xFFu) << 23); }
 
-template <int D>
-__device__ __forceinline__ float qw_attn_xor_rows(float v, bool largest) {
-    const float a = __shfl_xor(v, 16, 64);
-    v = largest ? fmaxf(v, a) : v + a;
-    const float b = __shfl_xor(v, 32, 64);
-    return largest ? fmaxf(v, b) : v + b;
+// E elements from `at` on of a row and head: into the output where the range is the whole, else with the range's maximum and sum into the workspace.
+template <int DT, int D, uint32_t E>
+__device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t part, uint32_t row, uint32_t head, uint32_t at, float* o, float best, float total, bool first) {
+    const uint64_t item = (uint64_t)row * a.q_heads + head;
+    if (a.parts > 1u) {
+        const uint64_t items = (uint64_t)a.rows * a.q_heads, place = part * items + item;
+        if (first) *(f2_t*)(a.part + a.parts * items * D + place * 2u) = f2_t{best, total};
+#pragma unroll
+        for (uint32_t e = 0; e < E; e += 4u) *(f4_t*)(a.part + place * D + at + e) = f4_t{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        return;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* const y = a.out + (uint64_t)row * a.ld_out + head * D + at;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
+#pragma unroll
+    for (uint32_t e = 0; e < E; e += E < 8u ? E : 8u) qw_attn_store<DT, (E < 8u ? E : 8u)>(y + e, o + e);
+    if (a.lse && first) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
 }
 
 // ------------------------------------------------------------------------------------------------
-// Four waves share a tile of 16 query rows (token and head of a group) and a range of tokens, a step of 32 tokens of its own each; all stays in registers.
-// S^T = K q^T, two operands of 16 tokens; the running maximum of a column (a query row) over the lanes of the wave; O^T += V^T P^T.
+// Few rows: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on
+// their way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T.
+// Elements become f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves
+// notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
+// two bf16 numbers each, a broken block of values for the rows alone that see its token.
 // ------------------------------------------------------------------------------------------------
 constexpr uint32_t QW_ATTN_TABLE = 1024;   // page numbers of a range that wait in LDS
+template <int D>
+struct qw_attn_shared {
+    int32_t table[QW_ATTN_TABLE];
+    float sums[4][16][D + 4];
+    float stats[4][16][2];
+};
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void qw_attn_stream_kernel(const qw_attn_args a) {
-    constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u, PITCH = D + 4u;   // ROWS: elements of a column's sum a lane has in one of 4
-    __shared__ int32_t table[QW_ATTN_TABLE];
-    __shared__ float sums[4][16][PITCH];
-    __shared__ float stats[4][16][2];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, i = lane & 15u, g = lane >> 4;
-    const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = rest / a.kv_heads, seq = blockIdx.y;
-    const qw_attn_seq s = qw_attn_sequence(a, seq);
-    const uint32_t count = s.n * a.shared, c0 = tile * 16u;
-    if (c0 >= count) return;
+__device__ __forceinline__ float qw_attn_max_rows(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// The columns c0 .. c0 + 15 over the tokens begin .. end - 1 (begin a multiple of 32).  Whether the range has to be done in the wide form (the same answer in every
+// wave); otherwise its results are written.  All waves of a workgroup call it, the first four work.
+template <int DT, int D, bool WIDE>
+__device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_attn_seq& s, uint32_t seq, uint32_t head, uint32_t part, uint32_t c0, uint32_t begin, uint32_t end,
+                                               qw_attn_shared<D>& sh) {
+    constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u;   // ROWS: accumulators, and elements of a column that a thread stores
+    constexpr int VT = WIDE ? QWHIP_BF16 : QWHIP_F16;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, i = lane & 15u, g = lane >> 4, count = s.n * a.shared;
+    qw_attn_range t = qw_attn_tokens<32>(a, s, c0, min(c0 + 15u, count - 1u), 0u);
+    t.first = max(t.first, begin), t.from = 0u, t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
     // this lane's column
     const uint32_t col = min(c0 + i, count - 1u), row = col / a.shared, member = col - row * a.shared;
-    const int32_t pos = (int32_t)(s.length - s.n + row);                                 // negative: sees nothing
-    const int32_t low = a.window && pos + 1 > (int32_t)a.window ? pos + 1 - (int32_t)a.window : 0;
-    // the tile's tokens: from its first row's first to its last row's last
-    const uint32_t row_a = c0 / a.shared, row_b = min(c0 + 15u, count - 1u) / a.shared;
-    const int32_t pos_a = (int32_t)(s.length - s.n + row_a), pos_b = (int32_t)(s.length - s.n + row_b);
-    const uint32_t low_a = a.window && pos_a + 1 > (int32_t)a.window ? (uint32_t)(pos_a + 1 - (int32_t)a.window) : 0u;
-    const uint32_t low_b = a.window && pos_b + 1 > (int32_t)a.window ? (uint32_t)(pos_b + 1 - (int32_t)a.window) : 0u;
-    const uint32_t first = low_a & ~31u, end = pos_b < 0 ? first : (uint32_t)pos_b + 1u;   // pos_b < 0: low_a is 0
-    const uint32_t steps = (end - first + 31u) / 32u, each = (steps + a.parts - 1u) / a.parts;
-    const uint32_t from = min(part * each, steps), to = min(from + each, steps);
+    const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
 
-    u4_t qf[SETS][WORDS];
+    u4_t q[SETS][WORDS];
     {
         const uint16_t* const x = a.q + (uint64_t)(s.row0 + row) * a.ld_q + (head * a.shared + member) * D;
 #pragma unroll
         for (uint32_t c = 0; c < SETS; ++c)
 #pragma unroll
-            for (uint32_t j = 0; j < WORDS; ++j) qf[c][j] = *(const u4_t*)(x + c * 128u + g * (8u * WORDS) + 8u * j);
+            for (uint32_t j = 0; j < WORDS; ++j) q[c][j] = *(const u4_t*)(x + c * 128u + g * (8u * WORDS) + 8u * j);
     }
     f4_t acc[ROWS];
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float top = -__builtin_inff(), sum = 0.0f;
+    float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of raw scores
+    bool far = false;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
 
     const uint32_t hold = ((QW_ATTN_TABLE - 1u) << a.geo.page_log2) >> 5;   // steps whose pages LDS holds, where they begin inside one too
-    for (uint32_t base = from; base < to; base += hold) {
-        const uint32_t stop = min(base + hold, to), first_page = (first + 32u * base) >> a.geo.page_log2;
-        const uint32_t last_page = min(first + 32u * stop - 1u, s.length - 1u) >> a.geo.page_log2;
+    for (uint32_t base = t.from; base < t.to; base += hold) {
+        const uint32_t stop = min(base + hold, t.to), first_page = (t.first + 32u * base) >> a.geo.page_log2;
+        const uint32_t last_page = min(t.first + 32u * stop - 1u, s.length - 1u) >> a.geo.page_log2;
         __syncthreads();
-        for (uint32_t p = tid; p <= last_page - first_page; p += 256u) {
-            const int32_t page = a.table[(uint64_t)seq * a.ld_table + first_page + p];
-            table[p] = (uint32_t)page < a.page_count ? page : 0;
+        for (uint32_t p = tid; p <= last_page - first_page; p += blockDim.x) {
+            const uint32_t page = (uint32_t)a.table[(uint64_t)seq * a.ld_table + first_page + p];
+            sh.table[p] = page < a.page_count ? (int32_t)page : 0;
         }
         __syncthreads();
+        if (wave >= 4u) continue;
         qw_attn_step<D> now, next;
-        if (base + wave < stop) qw_attn_load<D>(a, pages, stride, table, first_page, first + 32u * (base + wave), s.length, i, g, now);
+        if (base + wave < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t.first + 32u * (base + wave), s.length, i, g, now);
         for (uint32_t step = base + wave; step < stop; step += 4u) {
-            const uint32_t t0 = first + 32u * step;
-            if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, table, first_page, t0 + 128u, s.length, i, g, next);
-            uint32_t far_v = 0, far_k = 0;
+            const uint32_t t0 = t.first + 32u * step;
+            if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, next);
+            if constexpr (!WIDE) {
 #pragma unroll
-            for (uint32_t c = 0; c < SETS; ++c) {
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) far_v = max(far_v, ((now.v_scale[c][e >> 2] >> (8u * (e & 3u))) & 0xFFu) - QW_ATTN_F16_LEAST);
-                far_k = max(far_k, max(now.k_scale[0][c], now.k_scale[1][c]) - (DT == QWHIP_F16 ? QW_ATTN_F16_LEAST : 0u));
-                if constexpr (DT == QWHIP_F16) far_k = max(far_k, min(now.k_scale[0][c], now.k_scale[1][c]) - QW_ATTN_F16_LEAST);
+                for (uint32_t c = 0; c < SETS; ++c) far = far || qw_attn_far8(now.v_scale[c]) || qw_attn_far<DT>(now.k_scale[0][c]) || qw_attn_far<DT>(now.k_scale[1][c]);
             }
-            const bool plain = __ballot(far_v > QW_ATTN_F16_MOST - QW_ATTN_F16_LEAST ||
-                                        far_k > (DT == QWHIP_F16 ? QW_ATTN_F16_MOST - QW_ATTN_F16_LEAST : QW_ATTN_BF16_MOST)) == 0ull;
-            f4_t score[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
-            if (plain) {
+            f4_t x[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                    for (uint32_t c = 0; c < SETS; ++c) {
-                        const float unit = __uint_as_float(now.k_scale[h][c] << 23);
-#pragma unroll
-                        for (uint32_t j = 0; j < WORDS; ++j) score[h] = qw_attn_mfma<DT>(qw_attn_operand<DT>(now.k[h][c][j], unit), qf[c][j], score[h]);
-                    }
-            } else {
-                // keys in bf16, which holds every element; f16 queries as two bf16 numbers, which hold their eleven bits
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                    for (uint32_t c = 0; c < SETS; ++c) {
-                        const uint32_t byte = now.k_scale[h][c];
-                        const float unit = __uint_as_float((byte > QW_ATTN_BF16_MOST ? 127u : byte) << 23);
-#pragma unroll
-                        for (uint32_t j = 0; j < WORDS; ++j) {
-                            u4_t k = qw_attn_operand<QWHIP_BF16>(now.k[h][c][j], unit);
-                            if (byte > QW_ATTN_BF16_MOST) k = u4_t{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-                            if constexpr (DT == QWHIP_BF16) {
-                                score[h] = qw_attn_mfma<QWHIP_BF16>(k, qf[c][j], score[h]);
-                            } else {
-                                u4_t hi, lo;
-                                const h8_t x = __builtin_bit_cast(h8_t, qf[c][j]);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const float x0 = (float)x[2 * e], x1 = (float)x[2 * e + 1];
-                                    const uint32_t h0 = __float_as_uint(x0) & 0xFFFF0000u, h1 = __float_as_uint(x1) & 0xFFFF0000u;
-                                    hi[e] = (h0 >> 16) | h1;
-                                    // an infinity's or a NaN's rest is zero
-                                    const float l0 = (h0 & 0x7F800000u) == 0x7F800000u ? 0.0f : x0 - __uint_as_float(h0);
-                                    const float l1 = (h1 & 0x7F800000u) == 0x7F800000u ? 0.0f : x1 - __uint_as_float(h1);
-                                    lo[e] = (__float_as_uint(l0) >> 16) | (__float_as_uint(l1) & 0xFFFF0000u);
-                                }
-                                score[h] = qw_attn_mfma<QWHIP_BF16>(k, lo, score[h]);
-                                score[h] = qw_attn_mfma<QWHIP_BF16>(k, hi, score[h]);
-                            }
-                        }
-                    }
-            }
-            // masks where a column of the tile does not see the whole step
-            uint32_t seen = 0xFFu;
-            if ((int32_t)(t0 + 31u) > pos_a || t0 < low_b) {
-                seen = 0;
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) {
-                    const int32_t t = (int32_t)(t0 + 8u * g + e);
-                    const bool in = t <= pos && t >= low;
-                    seen |= in ? 1u << e : 0u;
-                    if (!in) score[e >> 2][e & 3u] = -__builtin_inff();
-                }
-            }
-            float most = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])), fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
-            most = qw_attn_xor_rows<D>(most, true);
-            const float larger = fmaxf(top, most), shift = larger == -__builtin_inff() ? 0.0f : larger * a.scale2;
-            const float fade = __builtin_amdgcn_exp2f(top * a.scale2 - shift);
-            float p[8];
-            float add = 0.0f;
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e >> 2][e & 3u], a.scale2, -shift));
-                add += p[e];
-            }
-            sum = sum * fade + add;
-            top = larger;
-#pragma unroll
-            for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
-            if (plain) {
-                u4_t w;
-                {
-                    h8_t x;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = (h1_t)p[e];
-                    w = __builtin_bit_cast(u4_t, x);
-                }
+            for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
                 for (uint32_t c = 0; c < SETS; ++c) {
-                    uint32_t x[8][4];   // [token][pair of elements]
+                    const bool nan = WIDE && now.k_scale[h][c] > QW_ATTN_BF16_MOST;
+                    const float unit = __uint_as_float((nan ? 127u : now.k_scale[h][c]) << 23);
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) {
-                        const float unit = __uint_as_float(((now.v_scale[c][e >> 2] >> (8u * (e & 3u))) & 0xFFu) << 23);
-                        const uint32_t word = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
-                        const u4_t o = qw_attn_operand<QWHIP_F16>(word, unit);
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) x[e][j] = o[j];
-                    }
-#pragma unroll
-                    for (uint32_t j = 0; j < (D == 64 ? 2u : 4u); ++j) {
-                        u4_t even, odd;
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            even[e] = __builtin_amdgcn_perm(x[2 * e + 1][j], x[2 * e][j], 0x05040100u);
-                            odd[e] = __builtin_amdgcn_perm(x[2 * e + 1][j], x[2 * e][j], 0x07060302u);
+                    for (uint32_t j = 0; j < WORDS; ++j) {
+                        u4_t k = qw_attn_operand<WIDE ? QWHIP_BF16 : DT>(now.k[h][c][j], unit);
+                        if (nan) k = u4_t{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+                        if constexpr (WIDE && DT == QWHIP_F16) {
+                            u4_t hi, lo;
+                            qw_attn_split(q[c][j], hi, lo);
+                            x[h] = qw_attn_mfma<QWHIP_BF16>(k, hi, qw_attn_mfma<QWHIP_BF16>(k, lo, x[h]));
+                        } else {
+                            x[h] = qw_attn_mfma<DT>(k, q[c][j], x[h]);
                         }
-                        acc[8 * c + 2 * j] = qw_attn_mfma<QWHIP_F16>(even, w, acc[8 * c + 2 * j]);
-                        acc[8 * c + 2 * j + 1] = qw_attn_mfma<QWHIP_F16>(odd, w, acc[8 * c + 2 * j + 1]);
                     }
                 }
+            // masks where a column does not see the whole step
+            uint32_t seen = 0xFFu;
+            if ((int32_t)(t0 + 31u) > t.pos_a || t0 < t.low_b) {
+                seen = 0u;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const int32_t at = (int32_t)(t0 + 8u * g + e);
+                    const bool in = at <= pos && at >= low;
+                    seen |= in ? 1u << e : 0u;
+                    if (!in) x[e >> 2][e & 3u] = -__builtin_inff();
+                }
+            }
+            const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+            // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
+            if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
+                const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
+                sum *= fade;
+#pragma unroll
+                for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
+                top = larger;
+            }
+            const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
+            float p[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
+            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            u4_t hi, lo, in;   // the weights; wide: as two bf16 numbers, and whether their tokens are seen
+            if constexpr (!WIDE) {
+                h8_t w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = (h1_t)p[e];
+                hi = __builtin_bit_cast(u4_t, w);
             } else {
-                // weights as two bf16 numbers (sixteen bits), values in bf16; a NaN block counts where a row sees its token
-                u4_t hi, lo, in;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     hi[e] = qw_attn_bf16x2(p[2 * e], p[2 * e + 1]);
                     lo[e] = qw_attn_bf16x2(p[2 * e] - __uint_as_float(hi[e] << 16), p[2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
-                    in[e] = ((seen >> (2 * e)) & 1u ? 0x3F80u : 0u) | ((seen >> (2 * e + 1)) & 1u ? 0x3F800000u : 0u);
+                    in[e] = ((seen >> (2 * e)) & 1u ? 0x3F80u : 0u) | ((seen >> (2 * e)) & 2u ? 0x3F800000u : 0u);
                 }
+            }
 #pragma unroll
-                for (uint32_t c = 0; c < SETS; ++c) {
-                    uint32_t x[8][4];
-                    u4_t broken = {0, 0, 0, 0};
+            for (uint32_t c = 0; c < SETS; ++c) {
+                uint32_t v[8][4];   // [token][pair of elements]
+                u4_t broken = {0, 0, 0, 0};
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) {
-                        const uint32_t byte = (now.v_scale[c][e >> 2] >> (8u * (e & 3u))) & 0xFFu;
-                        if (byte > QW_ATTN_BF16_MOST) broken[e >> 1] |= (e & 1u) ? 0x3F800000u : 0x3F80u;
-                        uint32_t word = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
-                        if (byte > QW_ATTN_BF16_MOST) word = 0u;
-                        const u4_t o = qw_attn_operand<QWHIP_BF16>(word, __uint_as_float((byte > QW_ATTN_BF16_MOST ? 127u : byte) << 23));
+                for (uint32_t e = 0; e < 8; ++e) {
+                    float unit = qw_attn_unit(now.v_scale[c], e);
+                    uint32_t word = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
+                    if (WIDE && __float_as_uint(unit) >> 23 > QW_ATTN_BF16_MOST) unit = 1.0f, word = 0u, broken[e >> 1] |= (e & 1u) ? 0x3F800000u : 0x3F80u;
+                    const u4_t o = qw_attn_operand<VT>(word, unit);
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) x[e][j] = o[j];
+                    for (uint32_t j = 0; j < 4; ++j) v[e][j] = o[j];
+                }
+                f4_t bad = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (WIDE) bad = qw_attn_mfma<QWHIP_BF16>(broken, in, bad);   // an accumulator's row is in one block in all of a set's
+#pragma unroll
+                for (uint32_t j = 0; j < (D == 64 ? 2u : 4u); ++j) {
+                    u4_t even, odd;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        even[e] = __builtin_amdgcn_perm(v[2 * e + 1][j], v[2 * e][j], 0x05040100u);
+                        odd[e] = __builtin_amdgcn_perm(v[2 * e + 1][j], v[2 * e][j], 0x07060302u);
                     }
-                    const f4_t bad = qw_attn_mfma<QWHIP_BF16>(broken, in, f4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                    for (uint32_t j = 0; j < (D == 64 ? 2u : 4u); ++j) {
-                        u4_t even, odd;
+                    for (uint32_t o = 0; o < 2; ++o) {
+                        f4_t& u = acc[8 * c + 2 * j + o];
+                        if constexpr (WIDE) u = qw_attn_mfma<VT>(o ? odd : even, lo, u);
+                        u = qw_attn_mfma<VT>(o ? odd : even, hi, u);
+                        if constexpr (WIDE) {
 #pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            even[e] = __builtin_amdgcn_perm(x[2 * e + 1][j], x[2 * e][j], 0x05040100u);
-                            odd[e] = __builtin_amdgcn_perm(x[2 * e + 1][j], x[2 * e][j], 0x07060302u);
+                            for (int r = 0; r < 4; ++r)
+                                if (bad[r] > 0.0f) u[r] = __builtin_nanf("");
                         }
-                        f4_t& u = acc[8 * c + 2 * j];
-                        f4_t& v = acc[8 * c + 2 * j + 1];
-                        u = qw_attn_mfma<QWHIP_BF16>(even, hi, qw_attn_mfma<QWHIP_BF16>(even, lo, u));
-                        v = qw_attn_mfma<QWHIP_BF16>(odd, hi, qw_attn_mfma<QWHIP_BF16>(odd, lo, v));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (bad[r] > 0.0f) u[r] = v[r] = __builtin_nanf("");
                     }
                 }
             }
             now = next;
         }
     }
+    if constexpr (!WIDE) {
+        if (__syncthreads_or(far ? 1 : 0)) return true;
+    } else {
+        __syncthreads();   // what an earlier range left in LDS has been read
+    }
 
-    // the four waves' columns, then the tile's rows
-    sum = qw_attn_xor_rows<D>(sum, false);
-    if (g == 0u) stats[wave][i][0] = top, stats[wave][i][1] = sum;
+    // the four waves' columns, then the columns' rows
+    if (wave < 4u) {
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (g == 0u) sh.stats[wave][i][0] = top, sh.stats[wave][i][1] = sum;
 #pragma unroll
-    for (uint32_t j = 0; j < ROWS; ++j)
+        for (uint32_t j = 0; j < ROWS; ++j)
 #pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            const uint32_t m = 4u * g + r;   // the accumulator's row
-            sums[wave][i][D == 64 ? 8u * (m & 7u) + 4u * (m >> 3) + j : 128u * (j >> 3) + 8u * m + (j & 7u)] = acc[j][r];
-        }
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint32_t m = 4u * g + r;   // the accumulator's row
+                sh.sums[wave][i][D == 64 ? 8u * (m & 7u) + 4u * (m >> 3) + j : 128u * (j >> 3) + 8u * m + (j & 7u)] = acc[j][r];
+            }
+    }
     __syncthreads();
     const uint32_t mine = tid >> 4, at = (tid & 15u) * ROWS;   // 16 threads a column, ROWS elements each
-    if (c0 + mine >= count) return;
+    if (wave >= 4u || c0 + mine >= count) return false;
     const uint32_t my_row = (c0 + mine) / a.shared, my_head = head * a.shared + (c0 + mine) - my_row * a.shared;
     float best = -__builtin_inff(), total = 0.0f, o[ROWS] = {};
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) best = fmaxf(best, stats[w][mine][0]);
+    for (uint32_t w = 0; w < 4; ++w) best = fmaxf(best, sh.stats[w][mine][0]);
     const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale2;
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(stats[w][mine][0] * a.scale2 - shift);
-        total += f * stats[w][mine][1];
+        const float f = __builtin_amdgcn_exp2f(sh.stats[w][mine][0] * a.scale2 - shift);
+        total += f * sh.stats[w][mine][1];
 #pragma unroll
-        for (uint32_t e = 0; e < ROWS; ++e) o[e] += f * sums[w][mine][at + e];
+        for (uint32_t e = 0; e < ROWS; ++e) o[e] += f * sh.sums[w][mine][at + e];
     }
-    const uint64_t item = (uint64_t)(s.row0 + my_row) * a.q_heads + my_head;
-    if (a.parts > 1u) {
-        const uint64_t items = (uint64_t)a.rows * a.q_heads, place = part * items + item;
-        float* const st = a.part + a.parts * items * D + place * 2u;
-        if (at == 0u) st[0] = best, st[1] = total;
+    qw_attn_write<DT, D, ROWS>(a, part, s.row0 + my_row, my_head, at, o, best, total, at == 0u);
+    return false;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void qw_attn_stream_kernel(const qw_attn_args a) {
+    __shared__ qw_attn_shared<D> sh;
+    const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = rest / a.kv_heads, seq = blockIdx.y;
+    const qw_attn_seq s = qw_attn_sequence(a, seq);
+    if (tile * 16u >= s.n * a.shared) return;
+    const qw_attn_range t = qw_attn_tokens<32>(a, s, tile * 16u, min(tile * 16u + 15u, s.n * a.shared - 1u), part);
+    const uint32_t begin = t.first + 32u * t.from, end = t.first + 32u * t.to;
+    if (qw_attn_stream<DT, D, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many rows: WAVES waves of 32 columns (query rows of a group of heads) each share tiles of T tokens.  A tile's codes are on their way while the tile before it
+// is contracted; the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane:
+// a conversion serves all columns of the workgroup.
+//   keys     operand of 32 tokens x 16 elements, lane (r, h) elements 8 h .. of token 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4: an accumulator's
+//            scores are then eight tokens in a row, twice, the operand of the weights
+//   values   operand of 32 elements x 16 tokens, lane (r, h) tokens 8 h .. of element 8 (r % W) + j, W = D / 8 words, r / W picking j in its tile
+// ------------------------------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
+    if constexpr (DT == QWHIP_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+
+template <int D, int WAVES>
+struct qw_attn_tile {
+    static constexpr uint32_t T = D == 256 ? 32 : 64, THREADS = WAVES * 64, W = D / 8, JT = 256 / D;
+    static constexpr uint32_t KW = T * W / THREADS;                              // words of a token that a thread turns
+    static constexpr uint32_t VS = T * D / 16 / THREADS ? T * D / 16 / THREADS : 1;   // pairs of elements of eight tokens' words
+    static constexpr uint32_t V_THREADS = T * D / 16 / VS;
+    static constexpr uint32_t K_BYTES = T * D * 2, BYTES = 2 * K_BYTES;
+};
+template <int D, int WAVES>
+struct qw_attn_fetch {
+    uint32_t k[qw_attn_tile<D, WAVES>::KW], k_scale;
+    u4_t v[2];
+    u2_t v_scale;
+};
+
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_args a) {
+    typedef qw_attn_tile<D, WAVES> L;
+    constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
+    __shared__ union {
+        uint8_t tile[2][L::BYTES];
+        qw_attn_shared<D> stream;
+    } sh;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = lane & 31u, hf = lane >> 5;
+    const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, part = rest % a.parts, tile = a.tiles - 1u - rest / a.parts, seq = blockIdx.y;
+    const qw_attn_seq s = qw_attn_sequence(a, seq);
+    const uint32_t count = s.n * a.shared, c0 = tile * (WAVES * 32u);
+    if (c0 >= count) return;
+    const qw_attn_range rg = qw_attn_tokens<T>(a, s, c0, min(c0 + WAVES * 32u - 1u, count - 1u), part);
+    // this lane's column
+    const uint32_t w0 = c0 + wave * 32u, col = min(w0 + r, count - 1u), row = col / a.shared, member = col - row * a.shared;
+    const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
+    const qw_attn_range mine = qw_attn_tokens<T>(a, s, min(w0, count - 1u), min(w0 + 31u, count - 1u), 0u);   // what the wave's columns see
+    const bool busy = w0 < count;
+    bool far = false;
+
+    u4_t q[KS];
+    {
+        const uint16_t* const x = a.q + (uint64_t)(s.row0 + row) * a.ld_q + (head * a.shared + member) * D;
 #pragma unroll
-        for (uint32_t e = 0; e < ROWS; e += 4u) *(f4_t*)(a.part + place * D + at + e) = f4_t{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        for (uint32_t j = 0; j < KS; ++j) q[j] = *(const u4_t*)(x + 16u * j + 8u * hf);
+    }
+    f16_t acc[NT];
+#pragma unroll
+    for (uint32_t j = 0; j < NT; ++j) acc[j] = f16_t{};
+    float top = -__builtin_inff(), sum = 0.0f;   // top: the running maximum that the weights stand under, of raw scores
+
+    // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
+    const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
+    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last8 = (s.length - 1u) & ~7u;   // read only where there are steps
+    const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
+    const uint32_t stride = a.kv_heads * a.geo.piece;
+    const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
+    auto token_k = [&](uint32_t step) { return min(rg.first + step * T + (kt & ~7u), last8); };
+    auto token_v = [&](uint32_t step) { return min(rg.first + step * T + vt, last8); };
+    auto page_of = [&](uint32_t token) {
+        const uint32_t p = (uint32_t)table[token >> a.geo.page_log2];
+        return p < a.page_count ? p : 0u;
+    };
+    auto fetch = [&](uint32_t step, uint32_t page_k, uint32_t page_v, qw_attn_fetch<D, WAVES>& f) {
+        const uint32_t t = (token_k(step) & inside) + (kt & 7u), t8 = (token_v(step) & inside) >> 3;
+        const uint8_t* const kp = pages + (uint64_t)page_k * stride;
+        const uint8_t* const vp = pages + (uint64_t)page_v * stride;
+        __builtin_memcpy(f.k, __builtin_assume_aligned(kp + t * (D / 2u) + kw * 4u, 4 * L::KW), 4 * L::KW);
+        f.k_scale = token_k(step) + (kt & 7u) >= s.length ? 127u : kp[a.geo.k_scales + t * (D / 32u) + kw / 4u];
+        const uint8_t* const w = vp + a.geo.v_codes + (t8 * W + vw) * 32u;
+        f.v[0] = *(const u4_t*)w;
+        f.v[1] = *(const u4_t*)(w + 16);
+        f.v_scale = qw_attn_tail(*(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + vw / 4u) * 8u), token_v(step), s.length);
+    };
+    auto turn = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t b) {
+        far = far || qw_attn_far<DT>(f.k_scale) || qw_attn_far8(f.v_scale);
+        const float unit = __uint_as_float(f.k_scale << 23);
+        const uint32_t t = kt & 31u, at = (t & 16u) | ((t & 4u) << 1) | ((t & 8u) >> 1) | (t & 3u);
+#pragma unroll
+        for (uint32_t i = 0; i < L::KW; ++i) {
+            const uint32_t w = kw + i;
+            *(u4_t*)(sh.tile[b] + ((((kt >> 5) * KS + (w >> 1)) * 64u) + (w & 1u) * 32u + at) * 16u) = qw_attn_operand<DT>(f.k[i], unit);
+        }
+        if (tid < L::V_THREADS) {
+#pragma unroll
+            for (uint32_t i = 0; i < L::VS; ++i) {
+                const uint32_t pair = vs + i;
+                uint32_t x[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    x[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(f.v[e >> 2][e & 3u] >> (8u * pair), qw_attn_unit(f.v_scale, e), 0));
+                u4_t even, odd;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    even[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
+                    odd[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+                }
+#pragma unroll
+                for (uint32_t o = 0; o < 2; ++o) {
+                    const uint32_t j = 2u * pair + o;
+                    *(u4_t*)(sh.tile[b] + L::K_BYTES + (((j / JT) * (T / 16u) + (vt >> 4)) * 64u + ((vt >> 3) & 1u) * 32u + vw + W * (j % JT)) * 16u) = o ? odd : even;
+                }
+            }
+        }
+    };
+
+    // scores of 32 tokens to weights: masks, the running maximum, exponentials, their sum
+    auto weights = [&](f16_t& x, uint32_t t0, bool mask) {
+        if (mask) {
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e) {
+                const int32_t t = (int32_t)(t0 + 16u * (e >> 3) + 8u * hf + (e & 7u));
+                if (t > pos || t < low) x[e] = -__builtin_inff();
+            }
+        }
+        float most = x[0];
+#pragma unroll
+        for (uint32_t e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
+        // a maximum that grew by less than 8 binary digits stays: weights up to 256 (the first one always grows)
+        if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            const float larger = fmaxf(top, most), shift = larger == -__builtin_inff() ? 0.0f : larger * a.scale2;
+            const float fade = __builtin_amdgcn_exp2f(top * a.scale2 - shift);
+            sum *= fade;
+#pragma unroll
+            for (uint32_t j = 0; j < NT; ++j) acc[j] = acc[j] * fade;
+            top = larger;
+        }
+        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
+#pragma unroll
+        for (uint32_t e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -shift));
+        sum += (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+    };
+    auto contract = [&](uint32_t b, uint32_t t0, bool mask) {
+        const uint8_t* const keys = sh.tile[b];
+        const uint8_t* const values = sh.tile[b] + L::K_BYTES;
+        f16_t x[HALVES];
+#pragma unroll
+        for (uint32_t h = 0; h < HALVES; ++h) {
+            x[h] = f16_t{};
+#pragma unroll
+            for (uint32_t j = 0; j < KS; ++j) x[h] = qw_attn_mfma32<DT>(*(const u4_t*)(keys + ((h * KS + j) * 64u + lane) * 16u), q[j], x[h]);
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < HALVES; ++h) {
+            weights(x[h], t0 + 32u * h, mask);
+#pragma unroll
+            for (uint32_t m = 0; m < 2; ++m) {
+                h8_t p;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) p[e] = (h1_t)x[h][8 * m + e];
+#pragma unroll
+                for (uint32_t j = 0; j < NT; ++j)
+                    acc[j] = qw_attn_mfma32<QWHIP_F16>(*(const u4_t*)(values + ((j * (T / 16u) + 2u * h + m) * 64u + lane) * 16u), __builtin_bit_cast(u4_t, p), acc[j]);
+            }
+        }
+    };
+
+    if (rg.from < rg.to) {
+        qw_attn_fetch<D, WAVES> f;
+        fetch(rg.from, page_of(token_k(rg.from)), page_of(token_v(rg.from)), f);
+        uint32_t next_k = page_of(token_k(min(rg.from + 1u, rg.to - 1u))), next_v = page_of(token_v(min(rg.from + 1u, rg.to - 1u)));
+        turn(f, rg.from & 1u);
+        __syncthreads();
+        for (uint32_t step = rg.from; step < rg.to; ++step) {
+            const uint32_t t0 = rg.first + step * T;
+            if (step + 1u < rg.to) {
+                fetch(step + 1u, next_k, next_v, f);
+                next_k = page_of(token_k(min(step + 2u, rg.to - 1u)));
+                next_v = page_of(token_v(min(step + 2u, rg.to - 1u)));
+            }
+            if (busy && (int32_t)t0 <= mine.pos_b && t0 + T > mine.low_a) contract(step & 1u, t0, (int32_t)(t0 + T - 1u) > mine.pos_a || t0 < mine.low_b);
+            if (step + 1u < rg.to) turn(f, (step + 1u) & 1u);
+            __syncthreads();
+        }
+    }
+    if (__syncthreads_or(far ? 1 : 0)) {
+        for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true>(a, s, seq, head, part, c, rg.first + rg.from * T, rg.first + rg.to * T, sh.stream);
         return;
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t* const y = a.out + (uint64_t)(s.row0 + my_row) * a.ld_out + my_head * D + at;
+
+    if (w0 + r >= count) return;
+    sum += __shfl_xor(sum, 32, 64);   // lanes r and r + 32 are the same column: both are here
+    // accumulator row m of tile j: element 8 (m % W) + JT j + m / W; a lane has whole words
+    constexpr uint32_t HALF = W / 2u;
 #pragma unroll
-    for (uint32_t e = 0; e < ROWS; ++e) {
-        const float x = o[e] * inv;
-        y[e] = DT == QWHIP_F16 ? __builtin_bit_cast(uint16_t, (h1_t)x) : qw_f32_to_bf16(x);
+    for (uint32_t e = 0; e < HALF; ++e) {
+        float o[8];
+#pragma unroll
+        for (uint32_t j = 0; j < NT; ++j)
+#pragma unroll
+            for (uint32_t k = 0; k < JT; ++k) o[JT * j + k] = acc[j][e + HALF * k];
+        qw_attn_write<DT, D, 8>(a, part, s.row0 + row, head * a.shared + member, 8u * (8u * (e >> 2) + 4u * hf + (e & 3u)), o, top, sum, e == 0u && hf == 0u);
     }
-    if (a.lse && at == 0u) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
 }
 
 // The parts of a row, joined in their order: a wave a row and head.
@@ -390,23 +630,34 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
         for (uint32_t e = 0; e < E; ++e) o[e] += f * x[e];
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t* const y = a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * E;
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-        const float x = o[e] * inv;
-        y[e] = DT == QWHIP_F16 ? __builtin_bit_cast(uint16_t, (h1_t)x) : qw_f32_to_bf16(x);
-    }
+    for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
+    qw_attn_store<DT, E>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * E, o);
     if (a.lse && lane == 0u) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
-static uint64_t qw_attn_tiles(const qwhip_kv_batch* b, uint32_t rows, uint32_t shared) { return ((uint64_t)(b->max_rows < rows ? b->max_rows : rows) * shared + 15u) / 16u; }
-// How many parts a call's rows are split into: workgroups for every compute unit four times over, at least two steps a wave.
-static uint32_t qw_attn_parts(uint64_t tiles, const qwhip_kv_batch* b, uint32_t window) {
-    if (tiles >= 1024u) return 1u;
+// The kernel of a call and how many parts its rows are split into.
+struct qw_attn_plan {
+    uint32_t waves;   // of the tile kernel; 0: the streaming kernel
+    uint64_t tiles;   // of a sequence and a head
+    uint32_t parts;
+};
+static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch* b, uint32_t rows, uint32_t q_heads, uint32_t window) {
+    const uint64_t columns = (uint64_t)(b->max_rows < rows ? b->max_rows : rows) * (q_heads / c->kv_heads);
+    qw_attn_plan p;
+    p.waves = columns <= 16u ? 0u : columns <= 128u || c->head_dim == 256u ? 4u : 8u;
+    if (getenv("QW_F")) p.waves = atoi(getenv("QW_F"));
+    const uint32_t across = p.waves ? p.waves * 32u : 16u;
+    p.tiles = (columns + across - 1u) / across;
+    const uint64_t all = p.tiles * c->kv_heads * b->seqs;
     const uint32_t longest = window && window < b->max_length && b->max_rows < b->max_length - window ? window + b->max_rows : b->max_length;
-    const uint32_t want = (uint32_t)((1024u + tiles - 1u) / tiles), most = (longest + 255u) / 256u;
-    return want < most ? want : most ? most : 1u;
+    uint64_t fill = p.waves == 8u ? 256u : p.waves ? 512u : 1024u;
+    if (getenv("QW_P")) fill = atoi(getenv("QW_P"));
+    const uint64_t want = all ? (fill + all - 1u) / all : 1u;
+    const uint32_t most = (longest + 255u) / 256u;
+    p.parts = want < most ? (uint32_t)want : most ? most : 1u;
+    return p;
 }
 static uint64_t qw_attn_part_bytes(uint32_t rows, uint32_t q_heads, uint32_t d) { return (uint64_t)rows * q_heads * (d + 2u) * 4u; }
 
@@ -426,14 +677,16 @@ static qwhip_status qw_attn_check(const qwhip_kv_cache* cache, const qwhip_kv_ba
 
 extern "C" uint64_t qwhip_kv_attention_workspace_bytes(const qwhip_kv_cache* cache, const qwhip_kv_batch* b, uint32_t q_heads, uint32_t rows, uint32_t window) {
     if (qw_attn_check(cache, b, q_heads, rows) != QWHIP_OK || rows == 0 || b->seqs == 0 || b->max_rows == 0) return 0;
-    const uint64_t tiles = qw_attn_tiles(b, rows, q_heads / cache->kv_heads) * cache->kv_heads * b->seqs;
-    const uint32_t parts = qw_attn_parts(tiles, b, window);
+    const uint32_t parts = qw_attn_choose(cache, b, rows, q_heads, window).parts;
     return parts > 1u ? parts * qw_attn_part_bytes(rows, q_heads, cache->head_dim) : 0u;
 }
 
 template <int DT, int D>
-static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t seqs) {
-    hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D>), dim3(a.parts * a.kv_heads * a.tiles, seqs), dim3(256), 0, s->stream, a);
+static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t waves, uint32_t seqs) {
+    const dim3 grid(a.parts * a.kv_heads * a.tiles, seqs);
+    if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D>), grid, dim3(256), 0, s->stream, a);
+    else if (waves == 4u) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4>), grid, dim3(256), 0, s->stream, a);
+    else if constexpr (D != 256) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 8>), grid, dim3(512), 0, s->stream, a);
     if (a.parts > 1u) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D>), dim3(qwhip_cdiv(a.max_rows * a.q_heads, 4u), seqs), dim3(256), 0, s->stream, a);
 }
 
@@ -458,8 +711,8 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     if (batch->max_length) QWHIP_REQUIRE(batch->block_table);
     if (((uintptr_t)q | (uintptr_t)out) & 15u) return qwhip_fail(QWHIP_E_BAD_SHAPE, "queries and output must be 16-byte aligned");
     const uint32_t shared = q_heads / cache->kv_heads, max_rows = batch->max_rows < rows ? batch->max_rows : rows;
-    const uint64_t tiles = qw_attn_tiles(batch, rows, shared);
-    if (tiles * cache->kv_heads > QW_ATTN_MOST_TILES) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of a sequence do not fit one launch", max_rows);
+    const qw_attn_plan plan = qw_attn_choose(cache, batch, rows, q_heads, window);
+    if (plan.tiles * cache->kv_heads * plan.parts > QW_ATTN_MOST_TILES) return qwhip_fail(QWHIP_E_BAD_SHAPE, "%u rows of a sequence do not fit one launch", max_rows);
     QW_ON_DEVICE_OF(s);
     qw_attn_args a = {};
     a.pages = (const uint8_t*)cache->pages;
@@ -468,19 +721,19 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     a.geo = qw_kv_geometry_of(cache);
     a.page_count = cache->page_count, a.kv_heads = cache->kv_heads, a.ld_table = batch->ld_table, a.max_rows = max_rows, a.max_length = batch->max_length;
     a.rows = rows, a.q_heads = q_heads, a.shared = shared, a.ld_q = ld_q, a.ld_out = ld_out, a.window = window > 0x7FFFFFFFu ? 0u : window;
-    a.tiles = (uint32_t)tiles;
+    a.tiles = (uint32_t)plan.tiles;
     a.scale = scale, a.scale2 = scale * 1.4426950408889634f;
     a.parts = 1;
     if (workspace) {
-        a.parts = qw_attn_parts(tiles * cache->kv_heads * batch->seqs, batch, a.window);
+        a.parts = plan.parts;
         const uint64_t fit = workspace_bytes / qw_attn_part_bytes(rows, q_heads, d);
         if (fit < a.parts) a.parts = fit > 1u ? (uint32_t)fit : 1u;
     }
 #define QW_ATTN(DT)                                                          \
     do {                                                                     \
-        if (d == 64u) qw_launch_attn<DT, 64>(s, a, batch->seqs);             \
-        else if (d == 128u) qw_launch_attn<DT, 128>(s, a, batch->seqs);      \
-        else qw_launch_attn<DT, 256>(s, a, batch->seqs);                     \
+        if (d == 64u) qw_launch_attn<DT, 64>(s, a, plan.waves, batch->seqs);             \
+        else if (d == 128u) qw_launch_attn<DT, 128>(s, a, plan.waves, batch->seqs);      \
+        else qw_launch_attn<DT, 256>(s, a, plan.waves, batch->seqs);                     \
     } while (0)
     if (dtype == QWHIP_F16) QW_ATTN(QWHIP_F16);
     else QW_ATTN(QWHIP_BF16);
