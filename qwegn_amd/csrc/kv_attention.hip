@@ -113,10 +113,17 @@ __device__ __forceinline__ u4_t qw_attn_operand(uint32_t w, float scale) {
     }
     return o;
 }
-template <int DT>
-__device__ __forceinline__ uint32_t qw_attn_pair(uint32_t w, float scale) {   // the two lowest
-    if constexpr (DT == QWHIP_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
-    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+template <int DT, int J>   // elements 2 J and 2 J + 1
+__device__ __forceinline__ uint32_t qw_attn_pair(uint32_t w, float scale) {
+    if constexpr (DT == QWHIP_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, J));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, J));
+}
+template <int N, typename F>   // f of 0 .. N - 1 as constants
+__device__ __forceinline__ void qw_attn_pairs(F f) {
+    if constexpr (N > 0) {
+        qw_attn_pairs<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
 }
 template <int DT>
 __device__ __forceinline__ f4_t qw_attn_mfma(u4_t a, u4_t b, f4_t c) {
@@ -247,8 +254,8 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
         if (base + wave < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t.first + 32u * (base + wave), s.length, i, g, now);
         for (uint32_t step = base + wave; step < stop; step += 4u) {
             const uint32_t t0 = t.first + 32u * step;
-            if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, next);
             if constexpr (!WIDE) {
+                if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, next);
 #pragma unroll
                 for (uint32_t c = 0; c < SETS; ++c) far = far || qw_attn_far8(now.v_scale[c]) || qw_attn_far<DT>(now.k_scale[0][c]) || qw_attn_far<DT>(now.k_scale[1][c]);
             }
@@ -314,26 +321,32 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
             }
 #pragma unroll
             for (uint32_t c = 0; c < SETS; ++c) {
-                uint32_t v[8][4];   // [token][pair of elements]
+                float unit[8];
+                uint32_t word[8];
                 u4_t broken = {0, 0, 0, 0};
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    float unit = qw_attn_unit(now.v_scale[c], e);
-                    uint32_t word = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
-                    if (WIDE && __float_as_uint(unit) >> 23 > QW_ATTN_BF16_MOST) unit = 1.0f, word = 0u, broken[e >> 1] |= (e & 1u) ? 0x3F800000u : 0x3F80u;
-                    const u4_t o = qw_attn_operand<VT>(word, unit);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) v[e][j] = o[j];
+                    unit[e] = qw_attn_unit(now.v_scale[c], e);
+                    word[e] = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
+                    if constexpr (WIDE) {
+                        const bool nan = __float_as_uint(unit[e]) >> 23 > QW_ATTN_BF16_MOST;
+                        unit[e] = nan ? 1.0f : unit[e];
+                        word[e] = nan ? 0u : word[e];
+                        broken[e >> 1] |= nan ? 0x3F80u << (16u * (e & 1u)) : 0u;
+                    }
                 }
                 f4_t bad = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (WIDE) bad = qw_attn_mfma<QWHIP_BF16>(broken, in, bad);   // an accumulator's row is in one block in all of a set's
+                qw_attn_pairs<D == 64 ? 2 : 4>([&](auto pair) {
+                    constexpr int j = decltype(pair)::value;
+                    uint32_t v[8];
 #pragma unroll
-                for (uint32_t j = 0; j < (D == 64 ? 2u : 4u); ++j) {
+                    for (uint32_t e = 0; e < 8; ++e) v[e] = qw_attn_pair<VT, j>(word[e], unit[e]);
                     u4_t even, odd;
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        even[e] = __builtin_amdgcn_perm(v[2 * e + 1][j], v[2 * e][j], 0x05040100u);
-                        odd[e] = __builtin_amdgcn_perm(v[2 * e + 1][j], v[2 * e][j], 0x07060302u);
+                        even[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05040100u);
+                        odd[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07060302u);
                     }
 #pragma unroll
                     for (uint32_t o = 0; o < 2; ++o) {
@@ -346,9 +359,10 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                                 if (bad[r] > 0.0f) u[r] = __builtin_nanf("");
                         }
                     }
-                }
+                });
             }
-            now = next;
+            if constexpr (!WIDE) now = next;
+            else if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, now);
         }
     }
     if constexpr (!WIDE) {
@@ -390,7 +404,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(256) void qw_attn_stream_kernel(const qw_attn_args a) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
     __shared__ qw_attn_shared<D> sh;
     const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = rest / a.kv_heads, seq = blockIdx.y;
     const qw_attn_seq s = qw_attn_sequence(a, seq);
@@ -606,34 +620,69 @@ __global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_
     }
 }
 
-// The parts of a row, joined in their order: a wave a row and head.
-template <int DT, int D>
+// The parts of a row and head, joined in their order: few parts by D / 4 threads, more by a workgroup, whose threads take every (1024 / D)th part and meet in LDS.
+constexpr uint32_t QW_ATTN_MOST_PARTS = 256, QW_ATTN_FEW_PARTS = 4;
+template <int DT, int D, bool FEW>
 __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a) {
-    constexpr uint32_t E = D / 64u;
-    const uint32_t lane = threadIdx.x & 63u, at = blockIdx.x * 4u + (threadIdx.x >> 6), seq = blockIdx.y;
+    constexpr uint32_t LANES = D / 4u, GROUPS = 256u / LANES;
+    __shared__ float weight[QW_ATTN_MOST_PARTS], fold[2][4];
+    __shared__ f4_t sums[FEW ? 1 : GROUPS][LANES];
+    const uint32_t tid = threadIdx.x, lane = tid % LANES, group = tid / LANES, at = FEW ? blockIdx.x * GROUPS + group : blockIdx.x, seq = blockIdx.y;
     const qw_attn_seq s = qw_attn_sequence(a, seq);
     const uint32_t row = at / a.q_heads;
     if (row >= s.n) return;
     const uint64_t items = (uint64_t)a.rows * a.q_heads, item = (uint64_t)s.row0 * a.q_heads + at;
     const float* const stats = a.part + a.parts * items * D + item * 2u;
-    float best = -__builtin_inff();
-    for (uint32_t p = lane; p < a.parts; p += 64u) best = fmaxf(best, stats[p * items * 2u]);
+    const float* const x = a.part + item * D + lane * 4u;
+    float best = -__builtin_inff(), total = 0.0f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (FEW) {
+        f2_t st[QW_ATTN_FEW_PARTS];
+        f4_t y[QW_ATTN_FEW_PARTS];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
-    const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale2;
-    float total = 0.0f, o[E] = {};
-    for (uint32_t p = 0; p < a.parts; ++p) {
-        const float f = __builtin_amdgcn_exp2f(stats[p * items * 2u] * a.scale2 - shift);
-        total += f * stats[p * items * 2u + 1u];
-        const float* const x = a.part + (p * items + item) * D + lane * E;
+        for (uint32_t p = 0; p < QW_ATTN_FEW_PARTS; ++p) {
+            const uint32_t from = min(p, a.parts - 1u);
+            st[p] = *(const f2_t*)(stats + from * items * 2u);
+            y[p] = *(const f4_t*)(x + from * items * D);
+        }
 #pragma unroll
-        for (uint32_t e = 0; e < E; ++e) o[e] += f * x[e];
+        for (uint32_t p = 0; p < QW_ATTN_FEW_PARTS; ++p) best = fmaxf(best, st[p][0]);
+        const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale2;
+#pragma unroll
+        for (uint32_t p = 0; p < QW_ATTN_FEW_PARTS; ++p) {
+            if (p >= a.parts) break;
+            const float f = __builtin_amdgcn_exp2f(st[p][0] * a.scale2 - shift);
+            total += f * st[p][1];
+            o += f * y[p];
+        }
+    } else {
+        const f2_t st = tid < a.parts ? *(const f2_t*)(stats + tid * items * 2u) : f2_t{-__builtin_inff(), 0.0f};
+        best = st[0];
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
+        if ((tid & 63u) == 0u) fold[0][tid >> 6] = best;
+        __syncthreads();
+        best = fmaxf(fmaxf(fold[0][0], fold[0][1]), fmaxf(fold[0][2], fold[0][3]));
+        const float f = __builtin_amdgcn_exp2f(st[0] * a.scale2 - (best == -__builtin_inff() ? 0.0f : best * a.scale2));
+        weight[tid] = f;
+        total = f * st[1];
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+        if ((tid & 63u) == 0u) fold[1][tid >> 6] = total;
+        __syncthreads();
+        total = (fold[1][0] + fold[1][1]) + (fold[1][2] + fold[1][3]);
+#pragma unroll 4
+        for (uint32_t p = group; p < a.parts; p += GROUPS) o += weight[p] * *(const f4_t*)(x + p * items * D);
+        sums[group][lane] = o;
+        __syncthreads();
+        if (group != 0u) return;
+#pragma unroll
+        for (uint32_t k = 1; k < GROUPS; ++k) o += sums[k][lane];
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
-    qw_attn_store<DT, E>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * E, o);
-    if (a.lse && lane == 0u) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
+    float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    qw_attn_store<DT, 4>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * 4u, y);
+    if (a.lse && tid % LANES == 0u) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
@@ -657,6 +706,7 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
     const uint64_t want = all ? (fill + all - 1u) / all : 1u;
     const uint32_t most = (longest + 255u) / 256u;
     p.parts = want < most ? (uint32_t)want : most ? most : 1u;
+    if (p.parts > QW_ATTN_MOST_PARTS) p.parts = QW_ATTN_MOST_PARTS;
     return p;
 }
 static uint64_t qw_attn_part_bytes(uint32_t rows, uint32_t q_heads, uint32_t d) { return (uint64_t)rows * q_heads * (d + 2u) * 4u; }
@@ -687,7 +737,9 @@ static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t wav
     if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D>), grid, dim3(256), 0, s->stream, a);
     else if (waves == 4u) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4>), grid, dim3(256), 0, s->stream, a);
     else if constexpr (D != 256) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 8>), grid, dim3(512), 0, s->stream, a);
-    if (a.parts > 1u) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D>), dim3(qwhip_cdiv(a.max_rows * a.q_heads, 4u), seqs), dim3(256), 0, s->stream, a);
+    const uint32_t items = a.max_rows * a.q_heads;
+    if (a.parts > QW_ATTN_FEW_PARTS) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, false>), dim3(items, seqs), dim3(256), 0, s->stream, a);
+    else if (a.parts > 1u) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, true>), dim3(qwhip_cdiv(items, 1024u / D), seqs), dim3(256), 0, s->stream, a);
 }
 
 extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_kv_cache* cache, const qwhip_kv_batch* batch, const void* q, uint32_t dtype,
