@@ -434,7 +434,7 @@ struct qw_attn_tile {
     static constexpr uint32_t KW = T * W / THREADS;                              // words of a token that a thread turns
     static constexpr uint32_t VS = T * D / 16 / THREADS ? T * D / 16 / THREADS : 1;   // pairs of elements of eight tokens' words
     static constexpr uint32_t V_THREADS = T * D / 16 / VS;
-    static constexpr uint32_t K_BYTES = T * D * 2, BYTES = 2 * K_BYTES;
+    static constexpr uint32_t K_BYTES = T * D * 2;
 };
 template <int D, int WAVES>
 struct qw_attn_fetch {
@@ -444,11 +444,13 @@ struct qw_attn_fetch {
 };
 
 template <int DT, int D, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_args a) {
+__global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw_attn_tile_kernel(const qw_attn_args a) {
     typedef qw_attn_tile<D, WAVES> L;
     constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
-    __shared__ union {
-        uint8_t tile[2][L::BYTES];
+    __shared__ union __attribute__((aligned(16))) {
+        struct {
+            uint8_t k[2][L::K_BYTES], v[2][L::K_BYTES];
+        } tile;
         qw_attn_shared<D> stream;
     } sh;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = lane & 31u, hf = lane >> 5;
@@ -481,32 +483,39 @@ __global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
     const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
-    auto token_k = [&](uint32_t step) { return min(rg.first + step * T + (kt & ~7u), last8); };
-    auto token_v = [&](uint32_t step) { return min(rg.first + step * T + vt, last8); };
-    auto page_of = [&](uint32_t token) {
-        const uint32_t p = (uint32_t)table[token >> a.geo.page_log2];
-        return p < a.page_count ? p : 0u;
-    };
-    auto fetch = [&](uint32_t step, uint32_t page_k, uint32_t page_v, qw_attn_fetch<D, WAVES>& f) {
-        const uint32_t t = (token_k(step) & inside) + (kt & 7u), t8 = (token_v(step) & inside) >> 3;
-        const uint8_t* const kp = pages + (uint64_t)page_k * stride;
-        const uint8_t* const vp = pages + (uint64_t)page_v * stride;
+    // where the keys of step + 1 and the values of step come from: what a turn leaves in LDS
+    const uint32_t last = max(rg.to, 1u) - 1u;
+    auto token_k = [&](uint32_t step) { return min(rg.first + min(step + 1u, last) * T + (kt & ~7u), last8); };
+    auto token_v = [&](uint32_t step) { return min(rg.first + min(step, last) * T + vt, last8); };
+    auto page_at = [&](uint32_t token) { return (uint32_t)table[token >> a.geo.page_log2]; };
+    auto fetch_k = [&](uint32_t token, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+        const uint32_t t = (token & inside) + (kt & 7u);
+        const uint8_t* const kp = pages + (uint64_t)(page < a.page_count ? page : 0u) * stride;
         __builtin_memcpy(f.k, __builtin_assume_aligned(kp + t * (D / 2u) + kw * 4u, 4 * L::KW), 4 * L::KW);
-        f.k_scale = token_k(step) + (kt & 7u) >= s.length ? 127u : kp[a.geo.k_scales + t * (D / 32u) + kw / 4u];
+        f.k_scale = kp[a.geo.k_scales + t * (D / 32u) + kw / 4u];
+    };
+    auto fetch_v = [&](uint32_t token, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+        const uint32_t t8 = (token & inside) >> 3;
+        const uint8_t* const vp = pages + (uint64_t)(page < a.page_count ? page : 0u) * stride;
         const uint8_t* const w = vp + a.geo.v_codes + (t8 * W + vw) * 32u;
         f.v[0] = *(const u4_t*)w;
         f.v[1] = *(const u4_t*)(w + 16);
-        f.v_scale = qw_attn_tail(*(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + vw / 4u) * 8u), token_v(step), s.length);
+        f.v_scale = *(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + vw / 4u) * 8u);
     };
-    auto turn = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t b) {
-        far = far || qw_attn_far<DT>(f.k_scale) || qw_attn_far8(f.v_scale);
-        const float unit = __uint_as_float(f.k_scale << 23);
+    auto turn_k = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
+        const uint32_t byte = token + (kt & 7u) >= s.length ? 127u : f.k_scale;   // behind the last token: a harmless scale
+        far = far || qw_attn_far<DT>(byte);
+        const float unit = __uint_as_float(byte << 23);
         const uint32_t t = kt & 31u, at = (t & 16u) | ((t & 4u) << 1) | ((t & 8u) >> 1) | (t & 3u);
 #pragma unroll
         for (uint32_t i = 0; i < L::KW; ++i) {
             const uint32_t w = kw + i;
-            *(u4_t*)(sh.tile[b] + ((((kt >> 5) * KS + (w >> 1)) * 64u) + (w & 1u) * 32u + at) * 16u) = qw_attn_operand<DT>(f.k[i], unit);
+            *(u4_t*)(sh.tile.k[slot] + ((((kt >> 5) * KS + (w >> 1)) * 64u) + (w & 1u) * 32u + at) * 16u) = qw_attn_operand<DT>(f.k[i], unit);
         }
+    };
+    auto turn_v = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
+        const u2_t scales = qw_attn_tail(f.v_scale, token, s.length);
+        far = far || qw_attn_far8(scales);
         if (tid < L::V_THREADS) {
 #pragma unroll
             for (uint32_t i = 0; i < L::VS; ++i) {
@@ -514,7 +523,7 @@ __global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_
                 uint32_t x[8];
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e)
-                    x[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(f.v[e >> 2][e & 3u] >> (8u * pair), qw_attn_unit(f.v_scale, e), 0));
+                    x[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(f.v[e >> 2][e & 3u] >> (8u * pair), qw_attn_unit(scales, e), 0));
                 u4_t even, odd;
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
@@ -524,29 +533,54 @@ __global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_
 #pragma unroll
                 for (uint32_t o = 0; o < 2; ++o) {
                     const uint32_t j = 2u * pair + o;
-                    *(u4_t*)(sh.tile[b] + L::K_BYTES + (((j / JT) * (T / 16u) + (vt >> 4)) * 64u + ((vt >> 3) & 1u) * 32u + vw + W * (j % JT)) * 16u) = o ? odd : even;
+                    *(u4_t*)(sh.tile.v[slot] + (((j / JT) * (T / 16u) + (vt >> 4)) * 64u + ((vt >> 3) & 1u) * 32u + vw + W * (j % JT)) * 16u) = o ? odd : even;
                 }
             }
         }
     };
 
-    // scores of 32 tokens to weights: masks, the running maximum, exponentials, their sum
-    auto weights = [&](f16_t& x, uint32_t t0, bool mask) {
-        if (mask) {
+    // a wave's scores of the next tile and its weights of this one
+    f16_t x[HALVES];
+    h8_t p[2 * HALVES];
+    auto sees = [&](uint32_t step) { return step < rg.to && busy && (int32_t)(rg.first + step * T) <= mine.pos_b && rg.first + (step + 1u) * T > mine.low_a; };
+    auto scores = [&](uint32_t step) {
+        const uint8_t* const keys = sh.tile.k[step & 1u];
 #pragma unroll
-            for (uint32_t e = 0; e < 16; ++e) {
-                const int32_t t = (int32_t)(t0 + 16u * (e >> 3) + 8u * hf + (e & 7u));
-                if (t > pos || t < low) x[e] = -__builtin_inff();
-            }
+        for (uint32_t h = 0; h < HALVES; ++h) x[h] = f16_t{};
+#pragma unroll
+        for (uint32_t j = 0; j < KS; ++j)
+#pragma unroll
+            for (uint32_t h = 0; h < HALVES; ++h) x[h] = qw_attn_mfma32<DT>(*(const u4_t*)(keys + ((h * KS + j) * 64u + lane) * 16u), q[j], x[h]);
+    };
+    auto outputs = [&](uint32_t step) {
+        const uint8_t* const values = sh.tile.v[step & 1u];
+#pragma unroll
+        for (uint32_t m = 0; m < 2 * HALVES; ++m)
+#pragma unroll
+            for (uint32_t j = 0; j < NT; ++j)
+                acc[j] = qw_attn_mfma32<QWHIP_F16>(*(const u4_t*)(values + ((j * (T / 16u) + m) * 64u + lane) * 16u), __builtin_bit_cast(u4_t, p[m]), acc[j]);
+    };
+    // masks, the running maximum, exponentials, their sum
+    auto weights = [&](uint32_t step) {
+        const uint32_t t0 = rg.first + step * T;
+        if ((int32_t)(t0 + T - 1u) > mine.pos_a || t0 < mine.low_b) {
+#pragma unroll
+            for (uint32_t h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) {
+                    const int32_t t = (int32_t)(t0 + 32u * h + 16u * (e >> 3) + 8u * hf + (e & 7u));
+                    if (t > pos || t < low) x[h][e] = -__builtin_inff();
+                }
         }
-        float most = x[0];
+        float most = x[0][0];
 #pragma unroll
-        for (uint32_t e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
-        // a maximum that grew by less than 8 binary digits stays: weights up to 256 (the first one always grows)
+        for (uint32_t h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, x[h][e]);
+        // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
         if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
-            const float larger = fmaxf(top, most), shift = larger == -__builtin_inff() ? 0.0f : larger * a.scale2;
-            const float fade = __builtin_amdgcn_exp2f(top * a.scale2 - shift);
+            const float larger = fmaxf(top, fmaxf(most, __shfl_xor(most, 32, 64)));
+            const float fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
             sum *= fade;
 #pragma unroll
             for (uint32_t j = 0; j < NT; ++j) acc[j] = acc[j] * fade;
@@ -554,52 +588,58 @@ __global__ __launch_bounds__(WAVES * 64) void qw_attn_tile_kernel(const qw_attn_
         }
         const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
 #pragma unroll
-        for (uint32_t e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -shift));
-        sum += (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
-    };
-    auto contract = [&](uint32_t b, uint32_t t0, bool mask) {
-        const uint8_t* const keys = sh.tile[b];
-        const uint8_t* const values = sh.tile[b] + L::K_BYTES;
-        f16_t x[HALVES];
-#pragma unroll
         for (uint32_t h = 0; h < HALVES; ++h) {
-            x[h] = f16_t{};
 #pragma unroll
-            for (uint32_t j = 0; j < KS; ++j) x[h] = qw_attn_mfma32<DT>(*(const u4_t*)(keys + ((h * KS + j) * 64u + lane) * 16u), q[j], x[h]);
-        }
+            for (uint32_t e = 0; e < 16; ++e) x[h][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[h][e], a.scale2, -shift));
 #pragma unroll
-        for (uint32_t h = 0; h < HALVES; ++h) {
-            weights(x[h], t0 + 32u * h, mask);
-#pragma unroll
-            for (uint32_t m = 0; m < 2; ++m) {
-                h8_t p;
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) p[e] = (h1_t)x[h][8 * m + e];
-#pragma unroll
-                for (uint32_t j = 0; j < NT; ++j)
-                    acc[j] = qw_attn_mfma32<QWHIP_F16>(*(const u4_t*)(values + ((j * (T / 16u) + 2u * h + m) * 64u + lane) * 16u), __builtin_bit_cast(u4_t, p), acc[j]);
-            }
+            for (uint32_t e = 0; e < 16; ++e) p[2 * h + (e >> 3)][e & 7u] = (h1_t)x[h][e];
+            sum += (((x[h][0] + x[h][1]) + (x[h][2] + x[h][3])) + ((x[h][4] + x[h][5]) + (x[h][6] + x[h][7]))) +
+                   (((x[h][8] + x[h][9]) + (x[h][10] + x[h][11])) + ((x[h][12] + x[h][13]) + (x[h][14] + x[h][15])));
         }
     };
+    // LDS is written and read in order, loads from memory go on
+#define QW_ATTN_MEET() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
     if (rg.from < rg.to) {
+        const bool late = WAVES == 8 && wave >= 4u;   // half a step behind, and its turns half a step ahead of its needs
         qw_attn_fetch<D, WAVES> f;
-        fetch(rg.from, page_of(token_k(rg.from)), page_of(token_v(rg.from)), f);
-        uint32_t next_k = page_of(token_k(min(rg.from + 1u, rg.to - 1u))), next_v = page_of(token_v(min(rg.from + 1u, rg.to - 1u)));
-        turn(f, rg.from & 1u);
-        __syncthreads();
-        for (uint32_t step = rg.from; step < rg.to; ++step) {
-            const uint32_t t0 = rg.first + step * T;
-            if (step + 1u < rg.to) {
-                fetch(step + 1u, next_k, next_v, f);
-                next_k = page_of(token_k(min(step + 2u, rg.to - 1u)));
-                next_v = page_of(token_v(min(step + 2u, rg.to - 1u)));
-            }
-            if (busy && (int32_t)t0 <= mine.pos_b && t0 + T > mine.low_a) contract(step & 1u, t0, (int32_t)(t0 + T - 1u) > mine.pos_a || t0 < mine.low_b);
-            if (step + 1u < rg.to) turn(f, (step + 1u) & 1u);
-            __syncthreads();
+        uint32_t ahead = late ? rg.from : rg.from - 1u;   // the step whose turn comes next is ahead + 1, but for the first tile's keys
+        {
+            const uint32_t tk = token_k(rg.from - 1u);
+            fetch_k(tk, page_at(tk), f);
+            turn_k(f, tk, rg.from & 1u);
         }
+        if (late) {
+            const uint32_t tk = token_k(rg.from), tv = token_v(rg.from);
+            fetch_k(tk, page_at(tk), f);
+            fetch_v(tv, page_at(tv), f);
+            turn_k(f, tk, (rg.from + 1u) & 1u);
+            turn_v(f, tv, rg.from & 1u);
+        }
+        ++ahead;
+        fetch_k(token_k(ahead), page_at(token_k(ahead)), f);
+        fetch_v(token_v(ahead), page_at(token_v(ahead)), f);
+        uint32_t next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
+        QW_ATTN_MEET();
+        if (sees(rg.from)) scores(rg.from);
+        if (late) QW_ATTN_MEET();
+        for (uint32_t step = rg.from; step < rg.to; ++step) {
+            const bool now = sees(step);
+            if (now) weights(step);
+            turn_k(f, token_k(ahead), (ahead + 1u) & 1u);
+            turn_v(f, token_v(ahead), ahead & 1u);
+            ++ahead;
+            fetch_k(token_k(ahead), next_k, f);
+            fetch_v(token_v(ahead), next_v, f);
+            next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
+            QW_ATTN_MEET();
+            if (now) outputs(step);
+            if (sees(step + 1u)) scores(step + 1u);
+            QW_ATTN_MEET();
+        }
+        if (WAVES == 8 && !late) QW_ATTN_MEET();
     }
+#undef QW_ATTN_MEET
     if (__syncthreads_or(far ? 1 : 0)) {
         for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true>(a, s, seq, head, part, c, rg.first + rg.from * T, rg.first + rg.to * T, sh.stream);
         return;
