@@ -158,16 +158,27 @@ __device__ __forceinline__ void qw_attn_store(uint16_t* y, const float* o) {
 // under 2^-124 and count as zero); bf16 up to 2^125.
 constexpr uint32_t QW_ATTN_F16_LEAST = 114, QW_ATTN_F16_MOST = 140, QW_ATTN_BF16_MOST = 252;
 template <int DT>
-__device__ __forceinline__ bool qw_attn_far(uint32_t byte) {
-    return DT == QWHIP_F16 ? byte - QW_ATTN_F16_LEAST > QW_ATTN_F16_MOST - QW_ATTN_F16_LEAST && byte != 0u : byte > QW_ATTN_BF16_MOST;
+__device__ __forceinline__ uint32_t qw_attn_far(uint32_t byte) {   // 1 or 0: added up without branches
+    if constexpr (DT == QWHIP_F16) return (uint32_t)(byte - QW_ATTN_F16_LEAST > QW_ATTN_F16_MOST - QW_ATTN_F16_LEAST) & (uint32_t)(byte != 0u);
+    else return (uint32_t)(byte > QW_ATTN_BF16_MOST);
 }
-__device__ __forceinline__ bool qw_attn_far8(u2_t scales) {
+// The same for eight bytes, four at a time: not zero for one that is over 140, or 1 .. 113.
+__device__ __forceinline__ uint32_t qw_attn_far8(u2_t scales) {
     uint32_t bad = 0;
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) bad |= qw_attn_far<QWHIP_F16>((scales[e >> 2] >> (8u * (e & 3u))) & 0xFFu) ? 1u : 0u;
-    return bad != 0u;
+    for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t b = scales[e], low = b & 0x7F7F7F7Fu;
+        const uint32_t over = b & (low + 0x73737373u);                                          // top bits: 128 + at least 13
+        const uint32_t under = ~b & ~(low + 0x0E0E0E0Eu) & (low + 0x7F7F7F7Fu);                  // no top bit, under 114, not zero
+        bad |= (over | under) & 0x80808080u;
+    }
+    return bad;
 }
-__device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) { return __uint_as_float(((scales[e >> 2] >> (8u * (e & 3u))) & 0xFFu) << 23); }
+// Byte e of eight as the scale of a conversion, which reads the exponent field alone.
+__device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
+    const uint32_t w = scales[e >> 2];
+    return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
+}
 
 // E elements from `at` on of a row and head: into the output where the range is the whole, else with the range's maximum and sum into the workspace.
 template <int DT, int D, uint32_t E>
@@ -216,7 +227,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                                                qw_attn_shared<D>& sh) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u;   // ROWS: accumulators, and elements of a column that a thread stores
     constexpr int VT = WIDE ? QWHIP_BF16 : QWHIP_F16;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, i = lane & 15u, g = lane >> 4, count = s.n * a.shared;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), i = lane & 15u, g = lane >> 4, count = s.n * a.shared;
     qw_attn_range t = qw_attn_tokens<32>(a, s, c0, min(c0 + 15u, count - 1u), 0u);
     t.first = max(t.first, begin), t.from = 0u, t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
     // this lane's column
@@ -235,7 +246,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
     float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of raw scores
-    bool far = false;
+    uint32_t far = 0;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
 
@@ -257,7 +268,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
             if constexpr (!WIDE) {
                 if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, next);
 #pragma unroll
-                for (uint32_t c = 0; c < SETS; ++c) far = far || qw_attn_far8(now.v_scale[c]) || qw_attn_far<DT>(now.k_scale[0][c]) || qw_attn_far<DT>(now.k_scale[1][c]);
+                for (uint32_t c = 0; c < SETS; ++c) far |= qw_attn_far8(now.v_scale[c]) | qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
             }
             f4_t x[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -329,7 +340,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                     unit[e] = qw_attn_unit(now.v_scale[c], e);
                     word[e] = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
                     if constexpr (WIDE) {
-                        const bool nan = __float_as_uint(unit[e]) >> 23 > QW_ATTN_BF16_MOST;
+                        const bool nan = ((__float_as_uint(unit[e]) >> 23) & 0xFFu) > QW_ATTN_BF16_MOST;
                         unit[e] = nan ? 1.0f : unit[e];
                         word[e] = nan ? 0u : word[e];
                         broken[e >> 1] |= nan ? 0x3F80u << (16u * (e & 1u)) : 0u;
@@ -366,7 +377,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
         }
     }
     if constexpr (!WIDE) {
-        if (__syncthreads_or(far ? 1 : 0)) return true;
+        if (__syncthreads_or((int)far)) return true;
     } else {
         __syncthreads();   // what an earlier range left in LDS has been read
     }
@@ -444,7 +455,7 @@ struct qw_attn_fetch {
 };
 
 template <int DT, int D, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw_attn_tile_kernel(const qw_attn_args a) {
+__global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
     typedef qw_attn_tile<D, WAVES> L;
     constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
     __shared__ union __attribute__((aligned(16))) {
@@ -453,7 +464,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
         } tile;
         qw_attn_shared<D> stream;
     } sh;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = lane & 31u, hf = lane >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), r = lane & 31u, hf = lane >> 5;
     const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, part = rest % a.parts, tile = a.tiles - 1u - rest / a.parts, seq = blockIdx.y;
     const qw_attn_seq s = qw_attn_sequence(a, seq);
     const uint32_t count = s.n * a.shared, c0 = tile * (WAVES * 32u);
@@ -464,7 +475,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
     const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
     const qw_attn_range mine = qw_attn_tokens<T>(a, s, min(w0, count - 1u), min(w0 + 31u, count - 1u), 0u);   // what the wave's columns see
     const bool busy = w0 < count;
-    bool far = false;
+    uint32_t far = 0;
 
     u4_t q[KS];
     {
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
     };
     auto turn_k = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
         const uint32_t byte = token + (kt & 7u) >= s.length ? 127u : f.k_scale;   // behind the last token: a harmless scale
-        far = far || qw_attn_far<DT>(byte);
+        far |= qw_attn_far<DT>(byte);
         const float unit = __uint_as_float(byte << 23);
         const uint32_t t = kt & 31u, at = (t & 16u) | ((t & 4u) << 1) | ((t & 8u) >> 1) | (t & 3u);
 #pragma unroll
@@ -515,8 +526,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
     };
     auto turn_v = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
         const u2_t scales = qw_attn_tail(f.v_scale, token, s.length);
-        far = far || qw_attn_far8(scales);
-        if (tid < L::V_THREADS) {
+        far |= qw_attn_far8(scales);
+        if (L::V_THREADS == L::THREADS || tid < L::V_THREADS) {
 #pragma unroll
             for (uint32_t i = 0; i < L::VS; ++i) {
                 const uint32_t pair = vs + i;
@@ -543,22 +554,30 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
     f16_t x[HALVES];
     h8_t p[2 * HALVES];
     auto sees = [&](uint32_t step) { return step < rg.to && busy && (int32_t)(rg.first + step * T) <= mine.pos_b && rg.first + (step + 1u) * T > mine.low_a; };
-    auto scores = [&](uint32_t step) {
-        const uint8_t* const keys = sh.tile.k[step & 1u];
+    // The matrix unit's part of a step: this tile's values under its weights (`out`), the next tile's scores.  Operands come from LDS AHEAD of their use.
+    auto products = [&](uint32_t step, auto out) {
+        constexpr int OUTS = decltype(out)::value ? 2 * HALVES * NT : 0, ALL = OUTS + KS * HALVES, AHEAD = 8;
+        const uint8_t* const values = sh.tile.v[step & 1u] + lane * 16u;
+        const uint8_t* const keys = sh.tile.k[(step + 1u) & 1u] + lane * 16u;
+        u4_t y[AHEAD];
+        auto load = [&](int n) { y[n % AHEAD] = n < OUTS ? *(const u4_t*)(values + ((n % NT) * (T / 16u) + n / NT) * 1024u) : *(const u4_t*)(keys + ((n - OUTS) % HALVES * KS + (n - OUTS) / HALVES) * 1024u); };
 #pragma unroll
         for (uint32_t h = 0; h < HALVES; ++h) x[h] = f16_t{};
 #pragma unroll
-        for (uint32_t j = 0; j < KS; ++j)
+        for (int n = 0; n < AHEAD; ++n) load(n);
 #pragma unroll
-            for (uint32_t h = 0; h < HALVES; ++h) x[h] = qw_attn_mfma32<DT>(*(const u4_t*)(keys + ((h * KS + j) * 64u + lane) * 16u), q[j], x[h]);
-    };
-    auto outputs = [&](uint32_t step) {
-        const uint8_t* const values = sh.tile.v[step & 1u];
+        for (int n = 0; n < ALL; ++n) {
+            if (n < OUTS) acc[n % NT] = qw_attn_mfma32<QWHIP_F16>(y[n % AHEAD], __builtin_bit_cast(u4_t, p[n / NT]), acc[n % NT]);
+            else x[(n - OUTS) % HALVES] = qw_attn_mfma32<DT>(y[n % AHEAD], q[(n - OUTS) / HALVES], x[(n - OUTS) % HALVES]);
+            if (n + AHEAD < ALL) load(n + AHEAD);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);   // reads of LDS, then one for each matrix instruction
 #pragma unroll
-        for (uint32_t m = 0; m < 2 * HALVES; ++m)
-#pragma unroll
-            for (uint32_t j = 0; j < NT; ++j)
-                acc[j] = qw_attn_mfma32<QWHIP_F16>(*(const u4_t*)(values + ((j * (T / 16u) + m) * 64u + lane) * 16u), __builtin_bit_cast(u4_t, p[m]), acc[j]);
+        for (int n = 0; n < ALL - AHEAD; ++n) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
     };
     // masks, the running maximum, exponentials, their sum
     auto weights = [&](uint32_t step) {
@@ -601,31 +620,26 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
 #define QW_ATTN_MEET() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
     if (rg.from < rg.to) {
-        const bool late = WAVES == 8 && wave >= 4u;   // half a step behind, and its turns half a step ahead of its needs
         qw_attn_fetch<D, WAVES> f;
-        uint32_t ahead = late ? rg.from : rg.from - 1u;   // the step whose turn comes next is ahead + 1, but for the first tile's keys
+        uint32_t ahead = rg.from;   // the step whose values, and whose next step's keys, are turned next
         {
             const uint32_t tk = token_k(rg.from - 1u);
             fetch_k(tk, page_at(tk), f);
             turn_k(f, tk, rg.from & 1u);
         }
-        if (late) {
-            const uint32_t tk = token_k(rg.from), tv = token_v(rg.from);
-            fetch_k(tk, page_at(tk), f);
-            fetch_v(tv, page_at(tv), f);
-            turn_k(f, tk, (rg.from + 1u) & 1u);
-            turn_v(f, tv, rg.from & 1u);
-        }
-        ++ahead;
         fetch_k(token_k(ahead), page_at(token_k(ahead)), f);
         fetch_v(token_v(ahead), page_at(token_v(ahead)), f);
         uint32_t next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
         QW_ATTN_MEET();
-        if (sees(rg.from)) scores(rg.from);
-        if (late) QW_ATTN_MEET();
+        if (sees(rg.from)) products(rg.from - 1u, std::false_type{});
         for (uint32_t step = rg.from; step < rg.to; ++step) {
             const bool now = sees(step);
-            if (now) weights(step);
+            if (now) {
+                weights(step);
+            } else {
+#pragma unroll
+                for (uint32_t m = 0; m < 2 * HALVES; ++m) p[m] = h8_t{};
+            }
             turn_k(f, token_k(ahead), (ahead + 1u) & 1u);
             turn_v(f, token_v(ahead), ahead & 1u);
             ++ahead;
@@ -633,14 +647,14 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 || WAVES == 8 ? 1 : 2) void qw
             fetch_v(token_v(ahead), next_v, f);
             next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
             QW_ATTN_MEET();
-            if (now) outputs(step);
-            if (sees(step + 1u)) scores(step + 1u);
+            __builtin_amdgcn_s_setprio(1);
+            if (now || sees(step + 1u)) products(step, std::true_type{});   // one of the two may be idle work at either end of the range
+            __builtin_amdgcn_s_setprio(0);
             QW_ATTN_MEET();
         }
-        if (WAVES == 8 && !late) QW_ATTN_MEET();
     }
 #undef QW_ATTN_MEET
-    if (__syncthreads_or(far ? 1 : 0)) {
+    if (__syncthreads_or((int)far)) {
         for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true>(a, s, seq, head, part, c, rg.first + rg.from * T, rg.first + rg.to * T, sh.stream);
         return;
     }
@@ -735,7 +749,7 @@ struct qw_attn_plan {
 static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch* b, uint32_t rows, uint32_t q_heads, uint32_t window) {
     const uint64_t columns = (uint64_t)(b->max_rows < rows ? b->max_rows : rows) * (q_heads / c->kv_heads);
     qw_attn_plan p;
-    p.waves = columns <= 16u ? 0u : columns <= 128u || c->head_dim == 256u ? 4u : 8u;
+    p.waves = columns <= 16u ? 0u : 4u;
     if (getenv("QW_F")) p.waves = atoi(getenv("QW_F"));
     const uint32_t across = p.waves ? p.waves * 32u : 16u;
     p.tiles = (columns + across - 1u) / across;
