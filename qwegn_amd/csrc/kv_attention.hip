@@ -68,31 +68,64 @@ struct qw_attn_step {
     u4_t v[SETS][2];
     u2_t v_scale[SETS];
 };
+// Where a lane's pieces are in a page, from the step's first token on.
 template <int D>
-__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t first_page, uint32_t t0,
-                                             uint32_t length, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
+struct qw_attn_place {
+    uint32_t k, k_scale, v, v_scale;
+    bool k_second, v_second;   // SMALL: of the step's second page
+    template <bool SMALL>
+    __device__ __forceinline__ void set(const qw_attn_args& a, uint32_t i, uint32_t g) {
+        const uint32_t kt = 8u * (i >> 2) + (i & 3u), word = D == 64 ? i & 7u : i;
+        k_second = SMALL && i >= 8u, v_second = SMALL && g >= 2u;
+        const uint32_t kp = k_second ? kt - 16u : kt, vp = v_second ? g - 2u : g;
+        k = kp * (D / 2u) + g * (4u * qw_attn_step<D>::WORDS);
+        k_scale = a.geo.k_scales + kp * (D / 32u) + (D == 64 ? g >> 1 : g);
+        v = a.geo.v_codes + (vp * (D / 8u) + word) * 32u;
+        v_scale = a.geo.v_scales + (vp * (D / 32u) + (word >> 2)) * 8u;
+    }
+};
+// The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two.  The page is the same for all lanes: scalar loads and addresses.
+template <int D, bool SMALL>
+__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t t0, uint32_t length,
+                                             const qw_attn_place<D>& at, qw_attn_step<D>& s) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS;
-    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last = length - 1u;
-    // of a group of eight tokens behind the last one's the last one's is read, and masked
-    const uint32_t kt = min(t0 + 8u * (i >> 2), last & ~7u) + (i & 3u), vt = min(t0 + 8u * g, last & ~7u);
-    const uint8_t* const kp = head + (uint64_t)(uint32_t)table[(kt >> a.geo.page_log2) - first_page] * stride;
-    const uint8_t* const vp = head + (uint64_t)(uint32_t)table[(vt >> a.geo.page_log2) - first_page] * stride;
+    const uint32_t in = t0 & ((1u << a.geo.page_log2) - 1u), page0 = (uint32_t)table[t0 >> a.geo.page_log2];
+    const uint8_t* const first = head + (uint64_t)(page0 < a.page_count ? page0 : 0u) * stride;
+    const uint8_t* kp = first;
+    const uint8_t* vp = first;
+    if constexpr (SMALL) {
+        const uint32_t page1 = (uint32_t)table[min(t0 + 16u, length - 1u) >> 4];   // a half behind the last token is read from the last page, and masked
+        const uint8_t* const second = head + (uint64_t)(page1 < a.page_count ? page1 : 0u) * stride;
+        kp = at.k_second ? second : first;
+        vp = at.v_second ? second : first;
+    }
+    const uint8_t* const kc = kp + in * (D / 2u);
+    const uint8_t* const ks = kp + in * (D / 32u);
+    const uint8_t* const vc = vp + in * (D / 2u);
+    const uint8_t* const vs = vp + in * (D / 32u);
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t t = (kt & inside) + 4u * h;
+    for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
         for (uint32_t c = 0; c < SETS; ++c) {
-            __builtin_memcpy(s.k[h][c], __builtin_assume_aligned(kp + t * (D / 2u) + c * 64u + g * (4u * WORDS), 4 * WORDS), 4 * WORDS);
-            s.k_scale[h][c] = kt + 4u * h > last ? 127u : kp[a.geo.k_scales + t * (D / 32u) + (D == 64 ? g >> 1 : 4u * c + g)];
+            __builtin_memcpy(s.k[h][c], __builtin_assume_aligned(kc + at.k + 4u * h * (D / 2u) + c * 64u, 4 * WORDS), 4 * WORDS);
+            s.k_scale[h][c] = ks[at.k_scale + 4u * h * (D / 32u) + 4u * c];
         }
-    }
-    const uint32_t t8 = (vt & inside) >> 3, word = D == 64 ? i & 7u : i;
 #pragma unroll
     for (uint32_t c = 0; c < SETS; ++c) {
-        const uint8_t* const w = vp + a.geo.v_codes + (t8 * (D / 8u) + 16u * c + word) * 32u;
-        s.v[c][0] = *(const u4_t*)w;
-        s.v[c][1] = *(const u4_t*)(w + 16);
-        s.v_scale[c] = qw_attn_tail(*(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + 4u * c + (word >> 2)) * 8u), vt, length);
+        s.v[c][0] = *(const u4_t*)(vc + at.v + c * 512u);
+        s.v[c][1] = *(const u4_t*)(vc + at.v + c * 512u + 16u);
+        s.v_scale[c] = *(const u2_t*)(vs + at.v_scale + c * 32u);
+    }
+}
+// Tokens behind the last one: harmless scales.
+template <int D>
+__device__ __forceinline__ void qw_attn_cut(uint32_t t0, uint32_t length, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
+#pragma unroll
+    for (uint32_t c = 0; c < qw_attn_step<D>::SETS; ++c) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h)
+            if (t0 + 8u * (i >> 2) + (i & 3u) + 4u * h >= length) s.k_scale[h][c] = 127u;
+        s.v_scale[c] = t0 + 8u * g >= length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(s.v_scale[c], t0 + 8u * g, length);
     }
 }
 
@@ -207,10 +240,8 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 // notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
 // two bf16 numbers each, a broken block of values for the rows alone that see its token.
 // ------------------------------------------------------------------------------------------------
-constexpr uint32_t QW_ATTN_TABLE = 1024;   // page numbers of a range that wait in LDS
 template <int D>
 struct qw_attn_shared {
-    int32_t table[QW_ATTN_TABLE];
     float sums[4][16][D + 4];
     float stats[4][16][2];
 };
@@ -222,7 +253,7 @@ __device__ __forceinline__ float qw_attn_max_rows(float v) {
 
 // The columns c0 .. c0 + 15 over the tokens begin .. end - 1 (begin a multiple of 32).  Whether the range has to be done in the wide form (the same answer in every
 // wave); otherwise its results are written.  All waves of a workgroup call it, the first four work.
-template <int DT, int D, bool WIDE>
+template <int DT, int D, bool SMALL, bool WIDE>
 __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_attn_seq& s, uint32_t seq, uint32_t head, uint32_t part, uint32_t c0, uint32_t begin, uint32_t end,
                                                qw_attn_shared<D>& sh) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u;   // ROWS: accumulators, and elements of a column that a thread stores
@@ -246,29 +277,22 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
     float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of raw scores
-    uint32_t far = 0;
+    uint32_t far = 0, far_k = 0;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
+    const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
+    qw_attn_place<D> place;
+    place.template set<SMALL>(a, i, g);
 
-    const uint32_t hold = ((QW_ATTN_TABLE - 1u) << a.geo.page_log2) >> 5;   // steps whose pages LDS holds, where they begin inside one too
-    for (uint32_t base = t.from; base < t.to; base += hold) {
-        const uint32_t stop = min(base + hold, t.to), first_page = (t.first + 32u * base) >> a.geo.page_log2;
-        const uint32_t last_page = min(t.first + 32u * stop - 1u, s.length - 1u) >> a.geo.page_log2;
-        __syncthreads();
-        for (uint32_t p = tid; p <= last_page - first_page; p += blockDim.x) {
-            const uint32_t page = (uint32_t)a.table[(uint64_t)seq * a.ld_table + first_page + p];
-            sh.table[p] = page < a.page_count ? (int32_t)page : 0;
-        }
-        __syncthreads();
-        if (wave >= 4u) continue;
-        qw_attn_step<D> now, next;
-        if (base + wave < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t.first + 32u * (base + wave), s.length, i, g, now);
-        for (uint32_t step = base + wave; step < stop; step += 4u) {
-            const uint32_t t0 = t.first + 32u * step;
+    auto one = [&](uint32_t t0, qw_attn_step<D>& now) {
+            if (t0 + 32u > s.length) qw_attn_cut<D>(t0, s.length, i, g, now);
             if constexpr (!WIDE) {
-                if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, next);
 #pragma unroll
-                for (uint32_t c = 0; c < SETS; ++c) far |= qw_attn_far8(now.v_scale[c]) | qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
+                for (uint32_t c = 0; c < SETS; ++c) {
+                    far |= qw_attn_far8(now.v_scale[c]);
+                    if constexpr (DT == QWHIP_F16) far |= qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
+                    else far_k = max(far_k, max(now.k_scale[0][c], now.k_scale[1][c]));
+                }
             }
             f4_t x[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -282,8 +306,9 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                         u4_t k = qw_attn_operand<WIDE ? QWHIP_BF16 : DT>(now.k[h][c][j], unit);
                         if (nan) k = u4_t{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
                         if constexpr (WIDE && DT == QWHIP_F16) {
-                            u4_t hi, lo;
-                            qw_attn_split(q[c][j], hi, lo);
+                            u4_t hi, lo, y = q[c][j];
+                            asm volatile("" : "+v"(y));   // split anew every time: the parts would take as many registers again
+                            qw_attn_split(y, hi, lo);
                             x[h] = qw_attn_mfma<QWHIP_BF16>(k, hi, qw_attn_mfma<QWHIP_BF16>(k, lo, x[h]));
                         } else {
                             x[h] = qw_attn_mfma<DT>(k, q[c][j], x[h]);
@@ -372,11 +397,28 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                     }
                 });
             }
-            if constexpr (!WIDE) now = next;
-            else if (step + 4u < stop) qw_attn_load<D>(a, pages, stride, sh.table, first_page, t0 + 128u, s.length, i, g, now);
+    };
+    if (wave < 4u && wave < t.to) {
+        // wave w has the steps w, w + 4, ..
+        auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), s.length, place, f); };
+        qw_attn_step<D> f[WIDE ? 1 : 2];
+        if constexpr (WIDE) {
+            for (uint32_t step = wave; step < t.to; step += 4u) {
+                load(step, f[0]);
+                one(t.first + 32u * step, f[0]);
+            }
+        } else {
+            load(wave, f[0]);
+            for (uint32_t step = wave; step < t.to; step += 8u) {
+                load(step + 4u, f[1]);
+                one(t.first + 32u * step, f[0]);
+                load(step + 8u, f[0]);
+                if (step + 4u < t.to) one(t.first + 32u * (step + 4u), f[1]);
+            }
         }
     }
     if constexpr (!WIDE) {
+        far |= qw_attn_far<QWHIP_BF16>(far_k);
         if (__syncthreads_or((int)far)) return true;
     } else {
         __syncthreads();   // what an earlier range left in LDS has been read
@@ -414,7 +456,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     return false;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool SMALL>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
     __shared__ qw_attn_shared<D> sh;
     const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = rest / a.kv_heads, seq = blockIdx.y;
@@ -422,7 +464,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
     if (tile * 16u >= s.n * a.shared) return;
     const qw_attn_range t = qw_attn_tokens<32>(a, s, tile * 16u, min(tile * 16u + 15u, s.n * a.shared - 1u), part);
     const uint32_t begin = t.first + 32u * t.from, end = t.first + 32u * t.to;
-    if (qw_attn_stream<DT, D, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
+    if (qw_attn_stream<DT, D, SMALL, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, SMALL, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -655,7 +697,11 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
     }
 #undef QW_ATTN_MEET
     if (__syncthreads_or((int)far)) {
-        for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true>(a, s, seq, head, part, c, rg.first + rg.from * T, rg.first + rg.to * T, sh.stream);
+        const uint32_t begin = rg.first + rg.from * T, end = rg.first + rg.to * T;
+        if (a.geo.page_log2 == 4u)
+            for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true, true>(a, s, seq, head, part, c, begin, end, sh.stream);
+        else
+            for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
         return;
     }
 
@@ -788,7 +834,8 @@ extern "C" uint64_t qwhip_kv_attention_workspace_bytes(const qwhip_kv_cache* cac
 template <int DT, int D>
 static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t waves, uint32_t seqs) {
     const dim3 grid(a.parts * a.kv_heads * a.tiles, seqs);
-    if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D>), grid, dim3(256), 0, s->stream, a);
+    if (waves == 0u && a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
+    else if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
     else if (waves == 4u) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4>), grid, dim3(256), 0, s->stream, a);
     else if constexpr (D != 256) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 8>), grid, dim3(512), 0, s->stream, a);
     const uint32_t items = a.max_rows * a.q_heads;
