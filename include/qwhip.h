@@ -588,8 +588,8 @@ qwhip_status qwhip_mxfp4_gemv(qwhip_stream_t s, const qwhip_mxfp4_view* w, const
  * between calls and only launch kernels (a call can be captured); no door uses the stream's scratch. */
 
 /* What a layer does to its heads, in this order, in fp32, every operation rounded by itself:
- *   norm      x_i = (x_i * r) * g_i, r = 1 / sqrt(mean(x^2) + eps) over the head; the squares are added as a tree (inside each eight
- *             i and i + 4, then 2, then 1; the eights by halves, padded with zeros to a power of two)
+ *   norm      x_i = (x_i * r) * g_i, r = 1 / sqrt(sum(x^2) * (1 / head_dim) + eps); the squares are added as a tree (inside each eight i
+ *             and i + 4, then 2, then 1; the eights by halves, padded with zeros to a power of two)
  *   rotation  the first rope_dims elements, a = x_i and b = x_{i + rope_dims / 2} (QWHIP_HEAD_ROPE_PAIRS: x_{2i} and x_{2i + 1}):
  *             a c - b s, b c + a s with c, s of the row's position
  *   FWHT-32   every 32 elements, as in qwhip_fwht32: queries and keys both (their product stays), values alone (the attention's

@@ -38,7 +38,7 @@ def heads(x, gamma=None, plus_one=False, eps=1e-6, cos_sin=None, position=None, 
             s = _halve((x * x).reshape(*x.shape[:-1], d // 8, 8))
             room = 1 << (d // 8 - 1).bit_length()
             s = _halve(np.concatenate([s, np.zeros((*s.shape[:-1], room - d // 8), dtype)], -1))
-            r = t(1.0) / np.sqrt(s / t(d) + t(np.float32(eps)))
+            r = t(1.0) / np.sqrt(s * (t(1.0) / t(d)) + t(np.float32(eps)))
             g = gamma.astype(dtype)
             x = (x * r[..., None]) * (t(1.0) + g if plus_one else g)
         if cos_sin is not None:

@@ -25,9 +25,7 @@ extern "C" qwhip_status qwhip_kv_cache_validate(const qwhip_kv_cache* c) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A head's elements lie eight to a lane: a quad of lanes holds a block of the transform and of the quantiser, 4 to 32 lanes a head.  The element that an
-// element turns with under the halves' rotation is loaded a second time (from the first-level cache) and normed beside it, so that nothing but the
-// norm's sum crosses lanes.  Every operation is rounded by itself, in a fixed order (the sum is a tree): keys next to a border of the 4-bit grid fall on
+// A head's elements lie eight to a lane: a quad of lanes holds a block of the transform and of the quantiser, 4 to 32 lanes a head.  Every operation is rounded by itself, in a fixed order (the sum is a tree): keys next to a border of the 4-bit grid fall on
 // the side that the definition in fp32 says, from either door and at every number of rows.
 // ------------------------------------------------------------------------------------------------
 struct qw_heads_side {
@@ -45,7 +43,7 @@ struct qw_heads_args {
     qw_kv_geometry geo;
     uint32_t rows, d, positions, rope, flags, slot_count;
     uint32_t across_log2;    // heads that a workgroup takes side by side
-    float eps;
+    float eps, inv_d;
 };
 
 // Lane l's value of lane l ^ N.
@@ -67,11 +65,35 @@ __device__ __forceinline__ float qw_sum_lanes(float v) {
     return v;
 }
 
-__device__ __forceinline__ void qw_head_gamma8(const h1_t* gamma, uint32_t at, bool plus_one, float r, float* v) {
-    float g[8];
+// Eight elements as they are in memory.
+template <int DT>
+struct qw_raw8 {
+    u4_t w[DT == QWHIP_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* x, uint64_t at) {
+        if constexpr (DT == QWHIP_F32) w[0] = *(const u4_t*)((const float*)x + at), w[1] = *(const u4_t*)((const float*)x + at + 4);
+        else w[0] = *(const u4_t*)((const uint16_t*)x + at);
+    }
+    __device__ __forceinline__ void floats(float* f) const { qw_load8_f32<DT>(w, 0, f); }
+};
+
+// What the head's normed elements are multiplied by.
+__device__ __forceinline__ void qw_head_gamma8(const h1_t* gamma, uint32_t at, bool plus_one, float* g) {
     qw_load8_f32<QWHIP_F16>(gamma, at, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (v[i] * r) * (plus_one ? 1.0f + g[i] : g[i]);
+    for (int i = 0; i < 8; ++i) g[i] = plus_one ? 1.0f + g[i] : g[i];
+}
+// Eight elements of an output row, streamed.
+template <int DT>
+__device__ __forceinline__ void qw_head_store8(void* dst, uint64_t at, const float* f) {
+    if constexpr (DT == QWHIP_BF16) {
+        typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+        b8_t o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (__bf16)f[i];
+        __builtin_nontemporal_store(__builtin_bit_cast(u4_t, o), (u4_t*)((uint16_t*)dst + at));
+    } else {
+        qw_stream8<DT>(dst, at, f);
+    }
 }
 
 template <int DT, int ODT, int LANES, bool CACHE>
@@ -86,8 +108,18 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
     }
     const uint32_t at = lane * 8u, half = a.rope / 2u;
     const bool there = at < a.d, turned = at < a.rope, pairs = (a.flags & QWHIP_HEAD_ROPE_PAIRS) != 0, second = !pairs && at >= half;
-    const uint32_t other = second ? at - half : at + half;
-    float c[8], s[8];
+    const int other = (int)((threadIdx.x & 63u) + (turned ? second ? 0u - half / 8u : half / 8u : 0u)) * 4;   // the lane of the elements that a lane's turn with
+    const uint32_t heads = a.q.heads + a.k.heads + a.v.heads, stride = gridDim.y * across;
+    qw_raw8<DT> raw = {};
+    auto load = [&](uint32_t h) {
+        const bool query = h < a.q.heads, value = CACHE && h >= a.q.heads + a.k.heads;
+        const uint32_t head = query ? h : value ? h - a.q.heads - a.k.heads : h - a.q.heads;
+        const qw_heads_side& side = query ? a.q : value ? a.v : a.k;
+        if (h < heads && there) raw.load(side.x, (uint64_t)row * side.ld + head * a.d + at);
+    };
+    uint32_t h = blockIdx.y * across + (slot & (across - 1u));
+    load(h);
+    float c[8], s[8], gq[8], gk[8];
     if (turned) {
         const int32_t p = max(0, min(a.position[row], (int32_t)a.positions - 1));
         const float* const t = a.cos_sin + (uint64_t)p * a.rope + (pairs ? at / 2u : second ? at - half : at);
@@ -98,44 +130,44 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
         } else {
             qw_load8_f32<QWHIP_F32>(t, 0, c);
             qw_load8_f32<QWHIP_F32>(t, half, s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = second ? s[i] : -s[i];   // a c + b (-s) is a c - b s, bit for bit
         }
     }
-    const uint32_t heads = a.q.heads + a.k.heads + a.v.heads;
-    for (uint32_t h = blockIdx.y * across + (slot & (across - 1u)); h < heads; h += gridDim.y * across) {
+    const bool plus_one = (a.flags & QWHIP_HEAD_GAMMA_PLUS_ONE) != 0;
+    if (there && a.q.gamma) qw_head_gamma8(a.q.gamma, at, plus_one, gq);
+    if (there && a.k.gamma) qw_head_gamma8(a.k.gamma, at, plus_one, gk);
+    for (; h < heads; h += stride) {
         const bool query = h < a.q.heads, value = CACHE && h >= a.q.heads + a.k.heads;
         const uint32_t head = query ? h : value ? h - a.q.heads - a.k.heads : h - a.q.heads;
-        const void* const x = query ? a.q.x : value ? a.v.x : a.k.x;
-        const h1_t* const gamma = query ? a.q.gamma : value ? nullptr : a.k.gamma;
-        const uint64_t from = (uint64_t)row * (query ? a.q.ld : value ? a.v.ld : a.k.ld) + head * a.d;
-        const bool rope = turned && !value;
-        float v[8] = {}, o[8];
-        if (there) qw_load8_f32<DT>(x, from + at, v);
-        if (rope && !pairs) qw_load8_f32<DT>(x, from + other, o);
-        if (gamma) {
+        const bool normed = query ? a.q.gamma != nullptr : !value && a.k.gamma != nullptr, rope = turned && !value;
+        float v[8];
+        raw.floats(v);
+        load(h + stride);   // the next head's elements on their way
+        if (normed) {
             float q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = v[i] * v[i];
             float sum = ((q[0] + q[4]) + (q[2] + q[6])) + ((q[1] + q[5]) + (q[3] + q[7]));
             sum = qw_sum_lanes<LANES>(sum);
-            const float r = 1.0f / sqrtf(sum / (float)a.d + a.eps);
-            const bool plus_one = (a.flags & QWHIP_HEAD_GAMMA_PLUS_ONE) != 0;
-            if (there) qw_head_gamma8(gamma, at, plus_one, r, v);
-            if (rope && !pairs) qw_head_gamma8(gamma, other, plus_one, r, o);
+            const float r = 1.0f / sqrtf(sum * a.inv_d + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (v[i] * r) * (query ? gq[i] : gk[i]);
         }
-        if (rope) {
-            if (pairs) {
+        if (a.rope && !pairs) {
+            float o[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x0 = v[2 * i], x1 = v[2 * i + 1];
-                    v[2 * i] = x0 * c[i] - x1 * s[i];
-                    v[2 * i + 1] = x1 * c[i] + x0 * s[i];
-                }
-            } else {
+            for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(other, __builtin_bit_cast(int, v[i])));
+            if (rope) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float turn = o[i] * s[i];
-                    v[i] = second ? v[i] * c[i] + turn : v[i] * c[i] - turn;
-                }
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] + o[i] * s[i];
+            }
+        } else if (rope) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                v[2 * i] = x0 * c[i] - x1 * s[i];
+                v[2 * i + 1] = x1 * c[i] + x0 * s[i];
             }
         }
         if (a.flags & (value ? QWHIP_HEAD_FWHT_V : QWHIP_HEAD_FWHT_QK)) qw_fwht32_quad(v, lane);
@@ -157,13 +189,14 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
             if (!out) continue;
             qw_e2m1_values8(w, qw_e8m0(byte), v);
         }
-        if (there) qw_stream8<ODT>(out, (uint64_t)row * side.ld_out + head * a.d + at, v);
+        if (there) qw_head_store8<ODT>(out, (uint64_t)row * side.ld_out + head * a.d + at, v);
     }
 }
 
 template <int DT, int ODT, bool CACHE>
 static void qw_launch_heads(qwhip_stream_t s, qw_heads_args& a) {
     const uint32_t lanes = a.d <= 32u ? 4u : a.d <= 64u ? 8u : a.d <= 128u ? 16u : 32u, slots = 256u / lanes, heads = a.q.heads + a.k.heads + a.v.heads;
+    a.inv_d = 1.0f / (float)a.d;
     a.across_log2 = 0;
     while ((1u << a.across_log2) < heads && (1u << a.across_log2) < slots) ++a.across_log2;
     const uint32_t across = 1u << a.across_log2, down = slots >> a.across_log2, groups = (heads + across - 1u) / across, steps = (a.rows + down - 1u) / down;

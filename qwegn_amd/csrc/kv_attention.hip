@@ -801,10 +801,11 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
     p.tiles = (columns + across - 1u) / across;
     const uint64_t all = p.tiles * c->kv_heads * b->seqs;
     const uint32_t longest = window && window < b->max_length && b->max_rows < b->max_length - window ? window + b->max_rows : b->max_length;
-    uint64_t fill = p.waves == 8u ? 256u : p.waves ? 512u : 1024u;
+    uint64_t fill = p.waves ? 512u : 256u;
     if (getenv("QW_P")) fill = atoi(getenv("QW_P"));
     const uint64_t want = all ? (fill + all - 1u) / all : 1u;
-    const uint32_t most = (longest + 255u) / 256u;
+    uint32_t least = 128u; if (getenv("QW_M")) least = atoi(getenv("QW_M"));
+    const uint32_t most = (longest + least - 1u) / least;
     p.parts = want < most ? (uint32_t)want : most ? most : 1u;
     if (p.parts > QW_ATTN_MOST_PARTS) p.parts = QW_ATTN_MOST_PARTS;
     return p;
