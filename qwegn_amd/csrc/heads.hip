@@ -43,6 +43,7 @@ struct qw_heads_args {
     qw_kv_geometry geo;
     uint32_t rows, d, positions, rope, flags, slot_count;
     uint32_t across_log2;    // heads that a workgroup takes side by side
+    uint32_t q_groups, k_groups;   // workgroups over a row's query heads, over its keys' (and values')
     float eps, inv_d;
 };
 
@@ -109,18 +110,20 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
     const uint32_t at = lane * 8u, half = a.rope / 2u;
     const bool there = at < a.d, turned = at < a.rope, pairs = (a.flags & QWHIP_HEAD_ROPE_PAIRS) != 0, second = !pairs && at >= half;
     const int other = (int)((threadIdx.x & 63u) + (turned ? second ? 0u - half / 8u : half / 8u : 0u)) * 4;   // the lane of the elements that a lane's turn with
-    const uint32_t heads = a.q.heads + a.k.heads + a.v.heads, stride = gridDim.y * across;
+    // queries, keys or values: a workgroup has one of them
+    const uint32_t kind = blockIdx.y < a.q_groups ? 0u : !CACHE || blockIdx.y < a.q_groups + a.k_groups ? 1u : 2u;
+    const qw_heads_side& side = kind == 0u ? a.q : kind == 1u ? a.k : a.v;
+    const uint32_t groups = kind == 0u ? a.q_groups : a.k_groups, stride = groups * across;
+    const bool value = CACHE && kind == 2u, rope = turned && !value;
+    const uint64_t from = (uint64_t)row * side.ld + at;
     qw_raw8<DT> raw = {};
-    auto load = [&](uint32_t h) {
-        const bool query = h < a.q.heads, value = CACHE && h >= a.q.heads + a.k.heads;
-        const uint32_t head = query ? h : value ? h - a.q.heads - a.k.heads : h - a.q.heads;
-        const qw_heads_side& side = query ? a.q : value ? a.v : a.k;
-        if (h < heads && there) raw.load(side.x, (uint64_t)row * side.ld + head * a.d + at);
+    auto load = [&](uint32_t head) {
+        if (head < side.heads && there) raw.load(side.x, from + head * a.d);
     };
-    uint32_t h = blockIdx.y * across + (slot & (across - 1u));
-    load(h);
-    float c[8], s[8], gq[8], gk[8];
-    if (turned) {
+    uint32_t head = (blockIdx.y - (kind == 0u ? 0u : kind == 1u ? a.q_groups : a.q_groups + a.k_groups)) * across + (slot & (across - 1u));
+    load(head);
+    float c[8], s[8], gamma[8];
+    if (rope) {
         const int32_t p = max(0, min(a.position[row], (int32_t)a.positions - 1));
         const float* const t = a.cos_sin + (uint64_t)p * a.rope + (pairs ? at / 2u : second ? at - half : at);
         if (pairs) {
@@ -135,16 +138,12 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
         }
     }
     const bool plus_one = (a.flags & QWHIP_HEAD_GAMMA_PLUS_ONE) != 0;
-    if (there && a.q.gamma) qw_head_gamma8(a.q.gamma, at, plus_one, gq);
-    if (there && a.k.gamma) qw_head_gamma8(a.k.gamma, at, plus_one, gk);
-    for (; h < heads; h += stride) {
-        const bool query = h < a.q.heads, value = CACHE && h >= a.q.heads + a.k.heads;
-        const uint32_t head = query ? h : value ? h - a.q.heads - a.k.heads : h - a.q.heads;
-        const bool normed = query ? a.q.gamma != nullptr : !value && a.k.gamma != nullptr, rope = turned && !value;
+    if (there && side.gamma) qw_head_gamma8(side.gamma, at, plus_one, gamma);
+    for (; head < side.heads; head += stride) {
         float v[8];
         raw.floats(v);
-        load(h + stride);   // the next head's elements on their way
-        if (normed) {
+        load(head + stride);   // the next head's elements on their way
+        if (side.gamma) {
             float q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = v[i] * v[i];
@@ -152,9 +151,9 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
             sum = qw_sum_lanes<LANES>(sum);
             const float r = 1.0f / sqrtf(sum * a.inv_d + a.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (v[i] * r) * (query ? gq[i] : gk[i]);
+            for (int i = 0; i < 8; ++i) v[i] = (v[i] * r) * gamma[i];
         }
-        if (a.rope && !pairs) {
+        if (a.rope && !pairs && !value) {
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(other, __builtin_bit_cast(int, v[i])));
@@ -171,9 +170,7 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
             }
         }
         if (a.flags & (value ? QWHIP_HEAD_FWHT_V : QWHIP_HEAD_FWHT_QK)) qw_fwht32_quad(v, lane);
-        const qw_heads_side& side = query ? a.q : value ? a.v : a.k;
-        void* const out = side.out;
-        if (CACHE && !query) {
+        if (CACHE && kind != 0u) {
             uint32_t w, byte;
             qw_mxfp4_code8(v, w, byte);
             if (!there) continue;
@@ -186,21 +183,28 @@ __global__ __launch_bounds__(256) void qw_heads_kernel(const qw_heads_args a) {
                 *(uint32_t*)(piece + t * (a.d / 2u) + lane * 4u) = w;
                 if ((lane & 3u) == 0u) piece[a.geo.k_scales + t * blocks + block] = (uint8_t)byte;
             }
-            if (!out) continue;
+            if (!side.out) continue;
             qw_e2m1_values8(w, qw_e8m0(byte), v);
         }
-        if (there) qw_head_store8<ODT>(out, (uint64_t)row * side.ld_out + head * a.d + at, v);
+        if (there) qw_head_store8<ODT>(side.out, (uint64_t)row * side.ld_out + head * a.d + at, v);
     }
 }
 
 template <int DT, int ODT, bool CACHE>
 static void qw_launch_heads(qwhip_stream_t s, qw_heads_args& a) {
-    const uint32_t lanes = a.d <= 32u ? 4u : a.d <= 64u ? 8u : a.d <= 128u ? 16u : 32u, slots = 256u / lanes, heads = a.q.heads + a.k.heads + a.v.heads;
+    const uint32_t lanes = a.d <= 32u ? 4u : a.d <= 64u ? 8u : a.d <= 128u ? 16u : 32u, slots = 256u / lanes, most = a.q.heads > a.k.heads ? a.q.heads : a.k.heads;
+    const uint32_t fewer = a.q.heads && a.q.heads < a.k.heads ? a.q.heads : a.k.heads ? a.k.heads : a.q.heads;
     a.inv_d = 1.0f / (float)a.d;
+    // Few rows: every head on its own lanes.  Many: heads after each other, so that a row's table entries and the gammas are loaded once; into the cache eight rows
+    // a workgroup, whose values' words of eight tokens meet in one L2.
+    const bool many = a.rows >= 2048u;
+    const uint32_t side_by_side = !many ? most : CACHE ? slots / 8u : fewer, each = !many ? 1u : CACHE ? 4u : most;
     a.across_log2 = 0;
-    while ((1u << a.across_log2) < heads && (1u << a.across_log2) < slots) ++a.across_log2;
-    const uint32_t across = 1u << a.across_log2, down = slots >> a.across_log2, groups = (heads + across - 1u) / across, steps = (a.rows + down - 1u) / down;
-    const dim3 grid(steps, steps >= 2048u ? 1u : groups), block(256);
+    while ((1u << a.across_log2) < side_by_side && (1u << a.across_log2) < slots) ++a.across_log2;
+    const uint32_t across = 1u << a.across_log2, down = slots >> a.across_log2, steps = (a.rows + down - 1u) / down;
+    a.q_groups = (a.q.heads + across * each - 1u) / (across * each);
+    a.k_groups = (a.k.heads + across * each - 1u) / (across * each);
+    const dim3 grid(steps, a.q_groups + a.k_groups * (CACHE ? 2u : 1u)), block(256);
     if (lanes == 8u) hipLaunchKernelGGL((qw_heads_kernel<DT, ODT, 8, CACHE>), grid, block, 0, s->stream, a);
     else if (lanes == 16u) hipLaunchKernelGGL((qw_heads_kernel<DT, ODT, 16, CACHE>), grid, block, 0, s->stream, a);
     else if (lanes == 32u) hipLaunchKernelGGL((qw_heads_kernel<DT, ODT, 32, CACHE>), grid, block, 0, s->stream, a);

@@ -237,17 +237,12 @@ __device__ __forceinline__ void qw_fwht32_quad(float* f, uint32_t lane) {
             }
         }
     }
-    const bool neg1 = (lane & 1u) != 0u, neg2 = (lane & 2u) != 0u;
+    // the partner's element plus or minus the lane's own: the product with a sign is exact, and the exchange rides on the addition
+    const float sg1 = (lane & 1u) ? -1.0f : 1.0f, sg2 = (lane & 2u) ? -1.0f : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float p = QW_DPP_F32(f[i], 0xB1);   // quad_perm [1,0,3,2]
-        f[i] = neg1 ? (p - f[i]) : (f[i] + p);
-    }
+    for (int i = 0; i < 8; ++i) f[i] = QW_DPP_F32(f[i], 0xB1) + f[i] * sg1;               // quad_perm [1,0,3,2]
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float p = QW_DPP_F32(f[i], 0x4E);   // quad_perm [2,3,0,1]
-        f[i] = (neg2 ? (p - f[i]) : (f[i] + p)) * QW_INV_SQRT32;
-    }
+    for (int i = 0; i < 8; ++i) f[i] = (QW_DPP_F32(f[i], 0x4E) + f[i] * sg2) * QW_INV_SQRT32;   // quad_perm [2,3,0,1]
 }
 
 // Eight floats as one 16-byte store of f16, or as two of fp32.
