@@ -496,7 +496,7 @@ struct qw_attn_fetch {
     u2_t v_scale;
 };
 
-template <int DT, int D, int WAVES>
+template <int DT, int D, int WAVES, bool BIG>
 __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
     typedef qw_attn_tile<D, WAVES> L;
     constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
@@ -532,31 +532,37 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
 
     // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
     const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
-    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last8 = (s.length - 1u) & ~7u;   // read only where there are steps
+    // A tile lies in one page, the same for all threads (BIG: scalar loads and addresses), or in several small ones.
+    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last_page = (s.length - 1u) >> a.geo.page_log2, last = max(rg.to, 1u) - 1u;   // read only where there are steps
+    const uint32_t kin = BIG ? kt : kt & inside, vin = BIG ? vt : vt & inside, kpage = BIG ? 0u : kt >> a.geo.page_log2, vpage = BIG ? 0u : vt >> a.geo.page_log2;
+    const uint32_t k_at = kin * (D / 2u) + kw * 4u, ks_at = a.geo.k_scales + kin * (D / 32u) + kw / 4u;
+    const uint32_t v_at = a.geo.v_codes + ((vin >> 3) * W + vw) * 32u, vs_at = a.geo.v_scales + ((vin >> 3) * (D / 32u) + vw / 4u) * 8u;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
     const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
-    // where the keys of step + 1 and the values of step come from: what a turn leaves in LDS
-    const uint32_t last = max(rg.to, 1u) - 1u;
-    auto token_k = [&](uint32_t step) { return min(rg.first + min(step + 1u, last) * T + (kt & ~7u), last8); };
-    auto token_v = [&](uint32_t step) { return min(rg.first + min(step, last) * T + vt, last8); };
-    auto page_at = [&](uint32_t token) { return (uint32_t)table[token >> a.geo.page_log2]; };
-    auto fetch_k = [&](uint32_t token, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
-        const uint32_t t = (token & inside) + (kt & 7u);
-        const uint8_t* const kp = pages + (uint64_t)(page < a.page_count ? page : 0u) * stride;
-        __builtin_memcpy(f.k, __builtin_assume_aligned(kp + t * (D / 2u) + kw * 4u, 4 * L::KW), 4 * L::KW);
-        f.k_scale = kp[a.geo.k_scales + t * (D / 32u) + kw / 4u];
+    auto tile_of = [&](uint32_t step) { return rg.first + min(step, last) * T; };   // first token; behind the last tile the last one's
+    auto page_at = [&](uint32_t t0, uint32_t more) {
+        const uint32_t p = (t0 >> a.geo.page_log2) + more;   // a part of a tile behind the last token is read from the last page, and masked
+        return (uint32_t)table[BIG ? p : min(p, last_page)];
     };
-    auto fetch_v = [&](uint32_t token, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
-        const uint32_t t8 = (token & inside) >> 3;
-        const uint8_t* const vp = pages + (uint64_t)(page < a.page_count ? page : 0u) * stride;
-        const uint8_t* const w = vp + a.geo.v_codes + (t8 * W + vw) * 32u;
+    auto base_of = [&](uint32_t page) { return pages + (uint64_t)(page < a.page_count ? page : 0u) * stride; };
+    auto fetch_k = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+        const uint8_t* const b = base_of(page);
+        const uint32_t in = BIG ? t0 & inside : 0u;
+        __builtin_memcpy(f.k, __builtin_assume_aligned(b + in * (D / 2u) + k_at, 4 * L::KW), 4 * L::KW);
+        f.k_scale = (b + in * (D / 32u))[ks_at];
+    };
+    auto fetch_v = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+        const uint8_t* const b = base_of(page);
+        const uint32_t in = BIG ? t0 & inside : 0u;
+        const uint8_t* const w = b + in * (D / 2u) + v_at;
         f.v[0] = *(const u4_t*)w;
         f.v[1] = *(const u4_t*)(w + 16);
-        f.v_scale = *(const u2_t*)(vp + a.geo.v_scales + (t8 * (D / 32u) + vw / 4u) * 8u);
+        f.v_scale = *(const u2_t*)(b + in * (D / 32u) + vs_at);
     };
-    auto turn_k = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
-        const uint32_t byte = token + (kt & 7u) >= s.length ? 127u : f.k_scale;   // behind the last token: a harmless scale
+    auto turn_k = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t t0, uint32_t slot) {
+        uint32_t byte = f.k_scale;
+        if (t0 + T > s.length) byte = t0 + kt >= s.length ? 127u : byte;   // behind the last token: a harmless scale
         far |= qw_attn_far<DT>(byte);
         const float unit = __uint_as_float(byte << 23);
         const uint32_t t = kt & 31u, at = (t & 16u) | ((t & 4u) << 1) | ((t & 8u) >> 1) | (t & 3u);
@@ -566,8 +572,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
             *(u4_t*)(sh.tile.k[slot] + ((((kt >> 5) * KS + (w >> 1)) * 64u) + (w & 1u) * 32u + at) * 16u) = qw_attn_operand<DT>(f.k[i], unit);
         }
     };
-    auto turn_v = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t token, uint32_t slot) {
-        const u2_t scales = qw_attn_tail(f.v_scale, token, s.length);
+    auto turn_v = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t t0, uint32_t slot) {
+        u2_t scales = f.v_scale;
+        if (t0 + T > s.length) scales = t0 + vt >= s.length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(scales, t0 + vt, s.length);
         far |= qw_attn_far8(scales);
         if (L::V_THREADS == L::THREADS || tid < L::V_THREADS) {
 #pragma unroll
@@ -663,15 +670,15 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
 
     if (rg.from < rg.to) {
         qw_attn_fetch<D, WAVES> f;
-        uint32_t ahead = rg.from;   // the step whose values, and whose next step's keys, are turned next
+        // a turn leaves the values of `step` and the keys of step + 1 in LDS
         {
-            const uint32_t tk = token_k(rg.from - 1u);
-            fetch_k(tk, page_at(tk), f);
-            turn_k(f, tk, rg.from & 1u);
+            const uint32_t t0 = tile_of(rg.from);
+            fetch_k(t0, page_at(t0, kpage), f);
+            turn_k(f, t0, rg.from & 1u);
         }
-        fetch_k(token_k(ahead), page_at(token_k(ahead)), f);
-        fetch_v(token_v(ahead), page_at(token_v(ahead)), f);
-        uint32_t next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
+        fetch_k(tile_of(rg.from + 1u), page_at(tile_of(rg.from + 1u), kpage), f);
+        fetch_v(tile_of(rg.from), page_at(tile_of(rg.from), vpage), f);
+        uint32_t next_k = page_at(tile_of(rg.from + 2u), kpage), next_v = page_at(tile_of(rg.from + 1u), vpage);
         QW_ATTN_MEET();
         if (sees(rg.from)) products(rg.from - 1u, std::false_type{});
         for (uint32_t step = rg.from; step < rg.to; ++step) {
@@ -682,12 +689,11 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
 #pragma unroll
                 for (uint32_t m = 0; m < 2 * HALVES; ++m) p[m] = h8_t{};
             }
-            turn_k(f, token_k(ahead), (ahead + 1u) & 1u);
-            turn_v(f, token_v(ahead), ahead & 1u);
-            ++ahead;
-            fetch_k(token_k(ahead), next_k, f);
-            fetch_v(token_v(ahead), next_v, f);
-            next_k = page_at(token_k(ahead + 1u)), next_v = page_at(token_v(ahead + 1u));
+            turn_k(f, tile_of(step + 1u), (step + 1u) & 1u);
+            turn_v(f, tile_of(step), step & 1u);
+            fetch_k(tile_of(step + 2u), next_k, f);
+            fetch_v(tile_of(step + 1u), next_v, f);
+            next_k = page_at(tile_of(step + 3u), kpage), next_v = page_at(tile_of(step + 2u), vpage);
             QW_ATTN_MEET();
             __builtin_amdgcn_s_setprio(1);
             if (now || sees(step + 1u)) products(step, std::true_type{});   // one of the two may be idle work at either end of the range
@@ -837,8 +843,8 @@ static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t wav
     const dim3 grid(a.parts * a.kv_heads * a.tiles, seqs);
     if (waves == 0u && a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
     else if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
-    else if (waves == 4u) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4>), grid, dim3(256), 0, s->stream, a);
-    else if constexpr (D != 256) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 8>), grid, dim3(512), 0, s->stream, a);
+    else if ((1u << a.geo.page_log2) >= qw_attn_tile<D, 4>::T) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4, true>), grid, dim3(256), 0, s->stream, a);
+    else hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4, false>), grid, dim3(256), 0, s->stream, a);
     const uint32_t items = a.max_rows * a.q_heads;
     if (a.parts > QW_ATTN_FEW_PARTS) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, false>), dim3(items, seqs), dim3(256), 0, s->stream, a);
     else if (a.parts > 1u) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, true>), dim3(qwhip_cdiv(items, 1024u / D), seqs), dim3(256), 0, s->stream, a);
