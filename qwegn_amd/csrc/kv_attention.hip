@@ -1,6 +1,5 @@
 // Attention over the paged MXFP4 cache.
 #include "qw_kv.h"
-#include <stdlib.h>
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
@@ -239,6 +238,10 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 // Elements become f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves
 // notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
 // two bf16 numbers each, a broken block of values for the rows alone that see its token.
+// Bound by the vector unit (conversions and exchanges of the elements: 96 of some 200 instructions a wave and step) and the bytes: a token of 64 sequences of up to 8192,
+// 40 heads of 128 over 8: 85 us = 4.7 TB/s; a token behind 131077: 34 us (29 and the join), 4.9 TB/s; behind 4096: 8.9 us, latency of two launches.  Steps on
+// the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last step
+// alone, two register sets in turn 85.  The four waves' sums meet in LDS at the end.
 // ------------------------------------------------------------------------------------------------
 template <int D>
 struct qw_attn_shared {
@@ -468,12 +471,20 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many rows: WAVES waves of 32 columns (query rows of a group of heads) each share tiles of T tokens.  A tile's codes are on their way while the tile before it
+// Many rows: four waves of 32 columns (query rows of a group of heads) each share tiles of 64 tokens (heads of 256: 32).  A tile's codes are on their way while the tile before it
 // is contracted; the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane:
 // a conversion serves all columns of the workgroup.
 //   keys     operand of 32 tokens x 16 elements, lane (r, h) elements 8 h .. of token 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4: an accumulator's
 //            scores are then eight tokens in a row, twice, the operand of the weights
 //   values   operand of 32 elements x 16 tokens, lane (r, h) tokens 8 h .. of element 8 (r % W) + j, W = D / 8 words, r / W picking j in its tile
+// A step: the weights of its tile out of its scores, the next tile turned into LDS, a meeting; its values under its weights and the next tile's scores, 32 matrix
+// instructions in a row whose operands come from LDS eight ahead; a meeting.  Bound by the vector unit beside the matrix unit (heads of 128: some 200 vector
+// instructions a wave and step against 32 matrix ones of 32 cycles), which the two workgroups of a compute unit overlap in part: 4096 rows of a prompt, 40 heads of
+// 128, bf16: 194 us = 885 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six ragged chunks of up to 700 rows behind up to 6001 tokens, 24
+// heads of 64, whose scores cost as much for half the products: 163 us = 470 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles
+// through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a wave's priority around them 204; scale bytes four at a time 201; pages and addresses
+// on the scalar unit 194.  Eight waves a workgroup turn a tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart
+// leave a SIMD's vector unit to one wave at a time (252); without the wide form behind it the kernel would take 5 % less.
 // ------------------------------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
@@ -481,24 +492,25 @@ __device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
 }
 
-template <int D, int WAVES>
+constexpr uint32_t QW_ATTN_WAVES = 4, QW_ATTN_COLUMNS = 32 * QW_ATTN_WAVES;
+template <int D>
 struct qw_attn_tile {
-    static constexpr uint32_t T = D == 256 ? 32 : 64, THREADS = WAVES * 64, W = D / 8, JT = 256 / D;
+    static constexpr uint32_t T = D == 256 ? 32 : 64, THREADS = QW_ATTN_WAVES * 64, W = D / 8, JT = 256 / D;
     static constexpr uint32_t KW = T * W / THREADS;                              // words of a token that a thread turns
     static constexpr uint32_t VS = T * D / 16 / THREADS ? T * D / 16 / THREADS : 1;   // pairs of elements of eight tokens' words
     static constexpr uint32_t V_THREADS = T * D / 16 / VS;
     static constexpr uint32_t K_BYTES = T * D * 2;
 };
-template <int D, int WAVES>
+template <int D>
 struct qw_attn_fetch {
-    uint32_t k[qw_attn_tile<D, WAVES>::KW], k_scale;
+    uint32_t k[qw_attn_tile<D>::KW], k_scale;
     u4_t v[2];
     u2_t v_scale;
 };
 
-template <int DT, int D, int WAVES, bool BIG>
-__global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
-    typedef qw_attn_tile<D, WAVES> L;
+template <int DT, int D, bool BIG>
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
+    typedef qw_attn_tile<D> L;
     constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
     __shared__ union __attribute__((aligned(16))) {
         struct {
@@ -509,9 +521,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), r = lane & 31u, hf = lane >> 5;
     const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, part = rest % a.parts, tile = a.tiles - 1u - rest / a.parts, seq = blockIdx.y;
     const qw_attn_seq s = qw_attn_sequence(a, seq);
-    const uint32_t count = s.n * a.shared, c0 = tile * (WAVES * 32u);
+    const uint32_t count = s.n * a.shared, c0 = tile * QW_ATTN_COLUMNS;
     if (c0 >= count) return;
-    const qw_attn_range rg = qw_attn_tokens<T>(a, s, c0, min(c0 + WAVES * 32u - 1u, count - 1u), part);
+    const qw_attn_range rg = qw_attn_tokens<T>(a, s, c0, min(c0 + QW_ATTN_COLUMNS - 1u, count - 1u), part);
     // this lane's column
     const uint32_t w0 = c0 + wave * 32u, col = min(w0 + r, count - 1u), row = col / a.shared, member = col - row * a.shared;
     const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
@@ -546,13 +558,13 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
         return (uint32_t)table[BIG ? p : min(p, last_page)];
     };
     auto base_of = [&](uint32_t page) { return pages + (uint64_t)(page < a.page_count ? page : 0u) * stride; };
-    auto fetch_k = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+    auto fetch_k = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D>& f) {
         const uint8_t* const b = base_of(page);
         const uint32_t in = BIG ? t0 & inside : 0u;
         __builtin_memcpy(f.k, __builtin_assume_aligned(b + in * (D / 2u) + k_at, 4 * L::KW), 4 * L::KW);
         f.k_scale = (b + in * (D / 32u))[ks_at];
     };
-    auto fetch_v = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D, WAVES>& f) {
+    auto fetch_v = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D>& f) {
         const uint8_t* const b = base_of(page);
         const uint32_t in = BIG ? t0 & inside : 0u;
         const uint8_t* const w = b + in * (D / 2u) + v_at;
@@ -560,7 +572,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
         f.v[1] = *(const u4_t*)(w + 16);
         f.v_scale = *(const u2_t*)(b + in * (D / 32u) + vs_at);
     };
-    auto turn_k = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t t0, uint32_t slot) {
+    auto turn_k = [&](const qw_attn_fetch<D>& f, uint32_t t0, uint32_t slot) {
         uint32_t byte = f.k_scale;
         if (t0 + T > s.length) byte = t0 + kt >= s.length ? 127u : byte;   // behind the last token: a harmless scale
         far |= qw_attn_far<DT>(byte);
@@ -572,7 +584,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
             *(u4_t*)(sh.tile.k[slot] + ((((kt >> 5) * KS + (w >> 1)) * 64u) + (w & 1u) * 32u + at) * 16u) = qw_attn_operand<DT>(f.k[i], unit);
         }
     };
-    auto turn_v = [&](const qw_attn_fetch<D, WAVES>& f, uint32_t t0, uint32_t slot) {
+    auto turn_v = [&](const qw_attn_fetch<D>& f, uint32_t t0, uint32_t slot) {
         u2_t scales = f.v_scale;
         if (t0 + T > s.length) scales = t0 + vt >= s.length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(scales, t0 + vt, s.length);
         far |= qw_attn_far8(scales);
@@ -669,7 +681,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
 #define QW_ATTN_MEET() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
     if (rg.from < rg.to) {
-        qw_attn_fetch<D, WAVES> f;
+        qw_attn_fetch<D> f;
         // a turn leaves the values of `step` and the keys of step + 1 in LDS
         {
             const uint32_t t0 = tile_of(rg.from);
@@ -705,9 +717,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 256 ? 1 : D == 128 ? 2 : 3) void q
     if (__syncthreads_or((int)far)) {
         const uint32_t begin = rg.first + rg.from * T, end = rg.first + rg.to * T;
         if (a.geo.page_log2 == 4u)
-            for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, true, true>(a, s, seq, head, part, c, begin, end, sh.stream);
+            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, true, true>(a, s, seq, head, part, c, begin, end, sh.stream);
         else
-            for (uint32_t c = c0; c < min(c0 + WAVES * 32u, count); c += 16u) qw_attn_stream<DT, D, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
+            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
         return;
     }
 
@@ -792,28 +804,33 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
-// The kernel of a call and how many parts its rows are split into.
+// The kernel of a call and how many parts its rows are split into.  Up to 16 columns (rows x heads of a group) the streaming kernel, else tiles of 128.
+// Parts give a launch that many workgroups (`fill`: one a compute unit for the streaming kernel, whose waves then have steps enough; two rounds of what the units
+// hold for the tile kernel), but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more:
+// a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 34 / 38 / 41 us, behind 500 in 1 / 4: 7.0 / 8.5; 64 sequences of up to 8192 in 1 / 2 / 4: 85 / 94 / 98;
+// 2048 rows of a prompt in 1 / 2: 65 / 95; 256 rows behind 16384 in 4 / 7 / 13 / 26: 145 / 158 / 139 / 169; six ragged chunks 1 / 2 / 3: 178 / 163 / 153;
+// windows of 8 rows over 1000 tokens, 32 tiles, in 1 / 2 / 8: 63 / 40 / 25.
 struct qw_attn_plan {
-    uint32_t waves;   // of the tile kernel; 0: the streaming kernel
+    bool stream;
     uint64_t tiles;   // of a sequence and a head
     uint32_t parts;
 };
 static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch* b, uint32_t rows, uint32_t q_heads, uint32_t window) {
     const uint64_t columns = (uint64_t)(b->max_rows < rows ? b->max_rows : rows) * (q_heads / c->kv_heads);
     qw_attn_plan p;
-    p.waves = columns <= 16u ? 0u : 4u;
-    if (getenv("QW_F")) p.waves = atoi(getenv("QW_F"));
-    const uint32_t across = p.waves ? p.waves * 32u : 16u;
-    p.tiles = (columns + across - 1u) / across;
+    p.stream = columns <= 16u;
+    p.tiles = p.stream ? 1u : (columns + QW_ATTN_COLUMNS - 1u) / QW_ATTN_COLUMNS;
     const uint64_t all = p.tiles * c->kv_heads * b->seqs;
     const uint32_t longest = window && window < b->max_length && b->max_rows < b->max_length - window ? window + b->max_rows : b->max_length;
-    uint64_t fill = p.waves ? 512u : 256u;
-    if (getenv("QW_P")) fill = atoi(getenv("QW_P"));
-    const uint64_t want = all ? (fill + all - 1u) / all : 1u;
-    uint32_t least = 128u; if (getenv("QW_M")) least = atoi(getenv("QW_M"));
-    const uint32_t most = (longest + least - 1u) / least;
-    p.parts = want < most ? (uint32_t)want : most ? most : 1u;
-    if (p.parts > QW_ATTN_MOST_PARTS) p.parts = QW_ATTN_MOST_PARTS;
+    const uint64_t fill = p.stream ? 256u : c->head_dim == 256u ? 512u : c->head_dim == 128u ? 1024u : 1536u;
+    const uint32_t least = p.stream || all <= 64u ? 128u : all <= 256u ? 512u : 2048u;   // tokens of a part
+    p.parts = 1u;
+    if (all < fill && longest > (p.stream ? 1024u : 512u)) {
+        const uint64_t want = (fill + all - 1u) / all;
+        const uint32_t most = (longest + least - 1u) / least;
+        p.parts = want < most ? (uint32_t)want : most;
+        if (p.parts > QW_ATTN_MOST_PARTS) p.parts = QW_ATTN_MOST_PARTS;
+    }
     return p;
 }
 static uint64_t qw_attn_part_bytes(uint32_t rows, uint32_t q_heads, uint32_t d) { return (uint64_t)rows * q_heads * (d + 2u) * 4u; }
@@ -839,12 +856,15 @@ extern "C" uint64_t qwhip_kv_attention_workspace_bytes(const qwhip_kv_cache* cac
 }
 
 template <int DT, int D>
-static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, uint32_t waves, uint32_t seqs) {
+static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, bool stream, uint32_t seqs) {
     const dim3 grid(a.parts * a.kv_heads * a.tiles, seqs);
-    if (waves == 0u && a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
-    else if (waves == 0u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
-    else if ((1u << a.geo.page_log2) >= qw_attn_tile<D, 4>::T) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4, true>), grid, dim3(256), 0, s->stream, a);
-    else hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, 4, false>), grid, dim3(256), 0, s->stream, a);
+    if (stream) {
+        if (a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
+        else hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
+    } else {
+        if ((1u << a.geo.page_log2) >= qw_attn_tile<D>::T) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
+        else hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
+    }
     const uint32_t items = a.max_rows * a.q_heads;
     if (a.parts > QW_ATTN_FEW_PARTS) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, false>), dim3(items, seqs), dim3(256), 0, s->stream, a);
     else if (a.parts > 1u) hipLaunchKernelGGL((qw_attn_join_kernel<DT, D, true>), dim3(qwhip_cdiv(items, 1024u / D), seqs), dim3(256), 0, s->stream, a);
@@ -891,9 +911,9 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     }
 #define QW_ATTN(DT)                                                          \
     do {                                                                     \
-        if (d == 64u) qw_launch_attn<DT, 64>(s, a, plan.waves, batch->seqs);             \
-        else if (d == 128u) qw_launch_attn<DT, 128>(s, a, plan.waves, batch->seqs);      \
-        else qw_launch_attn<DT, 256>(s, a, plan.waves, batch->seqs);                     \
+        if (d == 64u) qw_launch_attn<DT, 64>(s, a, plan.stream, batch->seqs);             \
+        else if (d == 128u) qw_launch_attn<DT, 128>(s, a, plan.stream, batch->seqs);      \
+        else qw_launch_attn<DT, 256>(s, a, plan.stream, batch->seqs);                     \
     } while (0)
     if (dtype == QWHIP_F16) QW_ATTN(QWHIP_F16);
     else QW_ATTN(QWHIP_BF16);
