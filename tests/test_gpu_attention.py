@@ -301,3 +301,45 @@ def test_pages_past_four_gigabytes(dev):
     assert np.array_equal(got, last.bytes)
     for b in (big, *bufs, out, xb, sb):
         b.free()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_many_rows_over_every_page(dev, page, d, t):
+    """Tiles in one page and over several, last tiles of every filling, ranges of a window that begin inside a page."""
+    c = Case(dev, page + d, d, 2, 3, page, [50, 129, 7, 64], [50, 517, 261, 64 + page // 2 + 3], t)
+    c.check(*c.run())
+    c.window = 77
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("d,rows", [(64, 1), (128, 1), (64, 40), (128, 90), (256, 33)])
+def test_a_part_in_the_wide_form_beside_others(dev, d, rows, page, t):
+    """Scales past the half types, and a broken block, in one place of a long sequence: the part that meets them covers its own tokens and no others."""
+    c = Case(dev, 91 + d, d, 2, 4, page, [rows, 1], [3001, 1500], t, std=0.5)
+    kc, ks, vc, vs = c.cache.planes()
+    for token, byte in ((1700, 100), (1733, 145 if t == "bf16" else 138), (2990, 255)):
+        p, o = c.table[0][token // page], token % page
+        vs[p, 0, o // 8, d // 32 - 1, o % 8] = byte
+    p, o = c.table[1][640 // page], 640 % page
+    ks[p, 1, o] = 96
+    y, l = c.run()
+    assert c.need > 0 and c.need // (c.total * 8 * (d + 2) * 4) > 1
+    c.check(y, l)
+    y0, l0 = c.run(room=0)
+    c.check(y0, l0)
+
+
+def test_a_sequence_longer_than_the_parts_there_are(dev):
+    c = Case(dev, 95, 64, 1, 2, 64, [2], [70000], "bf16", std=3.0)
+    c.check(*c.run())
+    assert c.need // (c.total * 2 * 66 * 4) == 256
+
+
+def test_group_of_one_and_the_largest_group(dev):
+    for shared, heads in ((1, 5), (64, 1)):
+        c = Case(dev, 96 + shared, 128, heads, shared, 16, [1, 3], [130, 260], "f16")
+        c.check(*c.run())

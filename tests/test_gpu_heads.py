@@ -280,3 +280,30 @@ def test_captured_and_on_two_streams(dev):
     for b in (xb, pb, qb, sb):
         b.free()
     rules.free()
+
+
+def test_append_with_queries_in_place_and_pitches(dev):
+    """A projection's rows as they are: queries turned in place, keys and values out of the same rows."""
+    d, qh, kh, page = 64, 6, 2, 16
+    for rows in (30, 2200):
+        rng = np.random.default_rng(rows)
+        rules = Rules(dev, rng, d, rows, 64, qwkv.PLUS_ONE | qwkv.FWHT_QK | qwkv.FWHT_V)
+        ld = (qh + 2 * kh) * d + 16
+        x = encode(rng.standard_normal((rows, ld)), "f16")
+        cache = qwkv.Cache(rows // page + 2, page, kh, d)
+        slots = rng.permutation(len(cache.bytes) * page)[:rows].astype(np.int32)
+        xb, sb, pb = dev.put(x), dev.put(slots), dev.put(cache.bytes)
+        view = qwhip.KvCache(pb.ptr, cache.bytes.nbytes, len(cache.bytes), page, kh, d)
+        k = xb.ptr + qh * d * 2
+        qwhip.check(dev.lib.qwhip_kv_append_mxfp4(dev.stream.handle, C.byref(view), C.byref(rules.c), rows, sb.ptr, k, ld, k + kh * d * 2, ld, qwhip.F16, xb.ptr, qh, ld, xb.ptr, ld,
+                                                  qwhip.F16, None, None))
+        dev.stream.sync()
+        val, got = decode(x, "f16"), xb.download(np.float16, x.shape)
+        part = lambda a, n: val[:, a * d:(a + n) * d].reshape(rows, n, d)  # noqa: E731
+        assert same(np.ascontiguousarray(got[:, : qh * d]).reshape(rows, qh, d), encode(rules.of(part(0, qh), "q"), "f16"), "f16")
+        assert np.array_equal(got[:, qh * d:], x[:, qh * d:])
+        cache.put(slots, rules.of(part(qh, kh), "k"), rules.of(part(qh + kh, kh), "v"))
+        assert np.array_equal(pb.download(np.uint8, cache.bytes.shape), cache.bytes)
+        for b in (xb, sb, pb):
+            b.free()
+        rules.free()
