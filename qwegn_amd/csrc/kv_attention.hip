@@ -17,16 +17,19 @@ struct qw_attn_args {
     float scale, scale2;   // scale2 = scale * log2(e)
 };
 
-// A sequence's rows and tokens, cut to what the host allows.
+// A sequence's rows and tokens, cut to what the host allows; the position of its first row.
 struct qw_attn_seq {
     uint32_t row0, n, length;
+    int32_t pos0;
 };
 __device__ __forceinline__ qw_attn_seq qw_attn_sequence(const qw_attn_args& a, uint32_t seq) {
     qw_attn_seq s;
     const int32_t from = a.row_start ? a.row_start[seq] : (int32_t)seq, to = a.row_start ? a.row_start[seq + 1u] : (int32_t)seq + 1;
     s.row0 = (uint32_t)max(0, min(from, (int32_t)a.rows));
-    s.n = min((uint32_t)max(0, min(to, (int32_t)a.rows) - (int32_t)s.row0), a.max_rows);
+    const int32_t n = max(0, min(to, (int32_t)a.rows) - (int32_t)s.row0);
+    s.n = min((uint32_t)n, a.max_rows);
     s.length = (uint32_t)max(0, min(a.lengths[seq], (int32_t)a.max_length));
+    s.pos0 = (int32_t)s.length - n;
     return s;
 }
 
@@ -42,7 +45,7 @@ __device__ __forceinline__ uint32_t qw_attn_low(const qw_attn_args& a, int32_t p
 template <uint32_t T>
 __device__ __forceinline__ qw_attn_range qw_attn_tokens(const qw_attn_args& a, const qw_attn_seq& s, uint32_t c0, uint32_t c1, uint32_t part) {
     qw_attn_range r;
-    r.pos_a = (int32_t)(s.length - s.n + c0 / a.shared), r.pos_b = (int32_t)(s.length - s.n + c1 / a.shared);
+    r.pos_a = s.pos0 + (int32_t)(c0 / a.shared), r.pos_b = s.pos0 + (int32_t)(c1 / a.shared);
     r.low_a = qw_attn_low(a, r.pos_a), r.low_b = qw_attn_low(a, r.pos_b);
     r.first = r.low_a & ~(T - 1u);
     const uint32_t end = r.pos_b < 0 ? r.first : (uint32_t)r.pos_b + 1u;   // pos_b < 0: low_a is 0
@@ -266,7 +269,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     t.first = max(t.first, begin), t.from = 0u, t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
     // this lane's column
     const uint32_t col = min(c0 + i, count - 1u), row = col / a.shared, member = col - row * a.shared;
-    const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
+    const int32_t pos = s.pos0 + (int32_t)row, low = (int32_t)qw_attn_low(a, pos);
 
     u4_t q[SETS][WORDS];
     {
@@ -527,7 +530,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_
     const qw_attn_range rg = qw_attn_tokens<T>(a, s, c0, min(c0 + QW_ATTN_COLUMNS - 1u, count - 1u), part);
     // this lane's column
     const uint32_t w0 = c0 + wave * 32u, col = min(w0 + r, count - 1u), row = col / a.shared, member = col - row * a.shared;
-    const int32_t pos = (int32_t)(s.length - s.n + row), low = (int32_t)qw_attn_low(a, pos);
+    const int32_t pos = s.pos0 + (int32_t)row, low = (int32_t)qw_attn_low(a, pos);
     const qw_attn_range mine = qw_attn_tokens<T>(a, s, min(w0, count - 1u), min(w0 + 31u, count - 1u), 0u);   // what the wave's columns see
     const bool busy = w0 < count;
     uint32_t far = 0;

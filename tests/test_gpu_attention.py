@@ -233,6 +233,20 @@ def test_bounds_of_the_host_cut(dev):
     assert bits((y, y2), (l, l2)) and not bits((full[0], y2))
 
 
+@pytest.mark.parametrize("bound", [1, 7, 20, 39])
+def test_rows_within_the_hosts_bound_keep_their_positions(dev, bound):
+    """A sequence of more rows than the host allowed: the ones that are done stand where they stood."""
+    c = Case(dev, 53, 64, 1, 2, 16, [10, 40], [100, 300], "bf16")
+    y, l = c.run()
+    got, lse = c.run(max_rows=bound)
+    for s, n in enumerate((10, 40)):
+        done, all_ = slice(c.start[s], c.start[s] + min(n, bound)), slice(c.start[s], c.start[s + 1])
+        left = slice(done.stop, all_.stop)
+        assert (got[left].view(np.uint16) == 0x7E01).all() and (lse[left].view(np.uint32) == 0x7E017E01).all()
+        y[done], l[done] = got[done], lse[done]
+    c.check(y, l)
+
+
 def test_captured_over_a_growing_sequence(dev):
     """A step's graph is captured at the largest length and replayed at all: lengths and rows live on the device."""
     c = Case(dev, 61, 128, 2, 5, 16, [1, 1], [900, 700], "bf16")
