@@ -215,6 +215,13 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
     return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
 }
 
+// What a row's sums are multiplied by, and the logarithm of its sum.  A row without a score over -inf has neither.  The largest score's own weight is one, so that a sum
+// of zero under a finite maximum means a scaled score over fp32's range: NaN.
+__device__ __forceinline__ float qw_attn_inverse(float best, float total) { return best == -__builtin_inff() && total == 0.0f ? 0.0f : 1.0f / total; }
+__device__ __forceinline__ float qw_attn_log(const qw_attn_args& a, float best, float total) {
+    return best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
+}
+
 // E elements from `at` on of a row and head: into the output where the range is the whole, else with the range's maximum and sum into the workspace.
 template <int DT, int D, uint32_t E>
 __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t part, uint32_t row, uint32_t head, uint32_t at, float* o, float best, float total, bool first) {
@@ -226,13 +233,13 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
         for (uint32_t e = 0; e < E; e += 4u) *(f4_t*)(a.part + place * D + at + e) = f4_t{o[e], o[e + 1], o[e + 2], o[e + 3]};
         return;
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = qw_attn_inverse(best, total);
     uint16_t* const y = a.out + (uint64_t)row * a.ld_out + head * D + at;
 #pragma unroll
     for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
 #pragma unroll
     for (uint32_t e = 0; e < E; e += E < 8u ? E : 8u) qw_attn_store<DT, (E < 8u ? E : 8u)>(y + e, o + e);
-    if (a.lse && first) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
+    if (a.lse && first) a.lse[item] = qw_attn_log(a, best, total);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -800,10 +807,10 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 #pragma unroll
         for (uint32_t k = 1; k < GROUPS; ++k) o += sums[k][lane];
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = qw_attn_inverse(best, total);
     float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     qw_attn_store<DT, 4>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * 4u, y);
-    if (a.lse && tid % LANES == 0u) a.lse[item] = best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
+    if (a.lse && tid % LANES == 0u) a.lse[item] = qw_attn_log(a, best, total);
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
@@ -882,7 +889,7 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     if (st != QWHIP_OK) return st;
     const uint32_t d = cache->head_dim;
     if (dtype != QWHIP_F16 && dtype != QWHIP_BF16) return qwhip_fail(QWHIP_E_BAD_SHAPE, "queries must be f16 or bf16, got dtype %u", dtype);
-    if (!(scale > 0.0f) || scale > 3.0e38f) return qwhip_fail(QWHIP_E_BAD_SHAPE, "scale must be positive and finite");
+    if (!(scale > 0.0f) || scale >= 0x1p127f) return qwhip_fail(QWHIP_E_BAD_SHAPE, "scale must be positive, under 2^127");
     if (ld_q == 0) ld_q = q_heads * d;
     if (ld_out == 0) ld_out = q_heads * d;
     if (ld_q < q_heads * d || ld_out < q_heads * d || ld_q % 8u != 0 || ld_out % 8u != 0)

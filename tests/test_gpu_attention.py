@@ -247,6 +247,21 @@ def test_rows_within_the_hosts_bound_keep_their_positions(dev, bound):
     c.check(y, l)
 
 
+@pytest.mark.parametrize("rows,lengths", [([1, 1], [40, 9]), ([1], [3000]), ([30, 2], [300, 17]), ([200], [2000])])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_scaled_scores_past_the_range(dev, rows, lengths, t):
+    """Every row has a scaled score over fp32's range, some have one below it: NaN, not a row of zeros."""
+    c = Case(dev, 54, 64, 2, 3, 32, rows, lengths, t, std=4.0, scale=1.6e38, noise=False)
+    y, l = c.run()
+    for s, n in enumerate(lengths):
+        a, b = c.start[s], c.start[s + 1]
+        k, _ = c.cache.tokens(c.table[s], n)
+        x = np.einsum("ihd,htd->iht", decode(c.q[a:b], t).astype(np.float64), np.repeat(k, 3, 0))
+        for i in range(b - a):
+            assert (x[i, :, : n - (b - a) + i + 1].max(axis=1) * 1.6e38 > 1.01 * 2.0 ** 128).all()
+        assert np.isnan(decode(y[a:b], t)).all() and np.isnan(l[a:b]).all()
+
+
 def test_captured_over_a_growing_sequence(dev):
     """A step's graph is captured at the largest length and replayed at all: lengths and rows live on the device."""
     c = Case(dev, 61, 128, 2, 5, 16, [1, 1], [900, 700], "bf16")

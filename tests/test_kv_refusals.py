@@ -137,6 +137,11 @@ def test_attention(lib, change, want):
     assert attention(lib, **change) == want, change
 
 
+@pytest.mark.parametrize("scale,want", [(2.0 ** -149, qwhip.OK), (2.0 ** 127 * 0.99, qwhip.OK), (2.0 ** 127 * 1.4, qwhip.E_BAD_SHAPE), (3.4e38, qwhip.E_BAD_SHAPE)])
+def test_scales_of_scores(lib, scale, want):
+    assert attention(lib, scale=scale, batch=batch(seqs=0)) == want
+
+
 def test_workspace_bytes(lib):
     size = lambda c=cache(), b=batch(), qh=4, rows=5, window=0: lib.qwhip_kv_attention_workspace_bytes(C.byref(c), C.byref(b), qh, rows, window)  # noqa: E731
     long = batch(seqs=1, max_rows=1, max_length=1 << 17, ld_table=1 << 13)
