@@ -492,7 +492,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
 // behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: some 200 vector
 // instructions a wave and step against 32 matrix ones of 32 cycles), which the two workgroups of a compute unit overlap in part: 4096 rows of a prompt, 40 heads of
 // 128, bf16: 194 us = 885 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six ragged chunks of up to 700 rows behind up to 6001 tokens, 24
-// heads of 64, whose scores cost as much for half the products: 163 us = 470 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles
+// heads of 64, whose scores cost as much for half the products, in three parts: 152 us = 500 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles
 // through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a wave's priority around them 204; scale bytes four at a time 201; pages and addresses
 // on the scalar unit 194 .. 204 by card; one meeting a step, not two 196.  Eight waves a workgroup turn a tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart
 // leave a SIMD's vector unit to one wave at a time (252); without the wide form behind it the kernel would take 5 % less.
@@ -815,8 +815,8 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
 // The kernel of a call and how many parts its rows are split into.  Up to 16 columns (rows x heads of a group) the streaming kernel, else tiles of 128.
-// Parts give a launch that many workgroups (`fill`: one a compute unit for the streaming kernel, whose waves then have steps enough; two rounds of what the units
-// hold for the tile kernel), but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more:
+// Parts give a launch that many workgroups (`fill`: one a compute unit for the streaming kernel, whose waves then have steps enough; two rounds and more of
+// what the units hold for the tile kernel), but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more:
 // a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 34 / 38 / 41 us, behind 500 in 1 / 4: 7.0 / 8.5; 64 sequences of up to 8192 in 1 / 2 / 4: 85 / 94 / 98;
 // 2048 rows of a prompt in 1 / 2: 65 / 95; 256 rows behind 16384 in 4 / 7 / 13 / 26: 145 / 158 / 139 / 169; six ragged chunks 1 / 2 / 3: 178 / 163 / 153;
 // windows of 8 rows over 1000 tokens, 32 tiles, in 1 / 2 / 8: 63 / 40 / 25; 16 rows behind 32768, 8 tiles, in 16 / 64 / 128: 59 / 36 / 48.
@@ -832,7 +832,7 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
     p.tiles = p.stream ? 1u : (columns + QW_ATTN_COLUMNS - 1u) / QW_ATTN_COLUMNS;
     const uint64_t all = p.tiles * c->kv_heads * b->seqs;
     const uint32_t longest = window && window < b->max_length && b->max_rows < b->max_length - window ? window + b->max_rows : b->max_length;
-    const uint64_t fill = p.stream ? 256u : c->head_dim == 256u ? 512u : c->head_dim == 128u ? 1024u : 1536u;
+    const uint64_t fill = p.stream ? 256u : c->head_dim == 256u ? 512u : c->head_dim == 128u ? 1024u : 2048u;
     const uint32_t eighth = longest / 8u;   // tokens of a part, at least: few tiles of a short sequence 128
     const uint32_t least = p.stream ? 128u : all > 256u ? 2048u : eighth < 128u ? 128u : eighth < 512u ? eighth : 512u;
     p.parts = 1u;
