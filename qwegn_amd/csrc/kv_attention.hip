@@ -1,5 +1,6 @@
 // Attention over the paged MXFP4 cache.
 #include "qw_kv.h"
+#include <algorithm>
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
@@ -243,7 +244,7 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 }
 
 // ------------------------------------------------------------------------------------------------
-// Few rows: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on
+// Streaming: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on
 // their way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T.
 // Elements become f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves
 // notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
@@ -472,7 +473,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 template <int DT, int D, bool SMALL>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
     __shared__ qw_attn_shared<D> sh;
-    const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = rest / a.kv_heads, seq = blockIdx.y;
+    const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = a.tiles - 1u - rest / a.kv_heads, seq = blockIdx.y;   // the last rows see the most: first
     const qw_attn_seq s = qw_attn_sequence(a, seq);
     if (tile * 16u >= s.n * a.shared) return;
     const qw_attn_range t = qw_attn_tokens<32>(a, s, tile * 16u, min(tile * 16u + 15u, s.n * a.shared - 1u), part);
@@ -481,8 +482,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many rows: four waves of 32 columns (query rows of a group of heads) each share tiles of 64 tokens (heads of 256: 32).  A tile's codes are on their way while the tile before it
-// is contracted; the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane:
+// Many rows, heads of 64 and 128: four waves of 32 columns each share tiles of 64 tokens.  A tile's codes are on their way while the tile before it is contracted; the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane:
 // a conversion serves all columns of the workgroup.
 //   keys     operand of 32 tokens x 16 elements, lane (r, h) elements 8 h .. of token 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4: an accumulator's
 //            scores are then eight tokens in a row, twice, the operand of the weights
@@ -506,10 +506,9 @@ __device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
 constexpr uint32_t QW_ATTN_WAVES = 4, QW_ATTN_COLUMNS = 32 * QW_ATTN_WAVES;
 template <int D>
 struct qw_attn_tile {
-    static constexpr uint32_t T = D == 256 ? 32 : 64, THREADS = QW_ATTN_WAVES * 64, W = D / 8, JT = 256 / D;
-    static constexpr uint32_t KW = T * W / THREADS;                              // words of a token that a thread turns
-    static constexpr uint32_t VS = T * D / 16 / THREADS ? T * D / 16 / THREADS : 1;   // pairs of elements of eight tokens' words
-    static constexpr uint32_t V_THREADS = T * D / 16 / VS;
+    static constexpr uint32_t T = 64, THREADS = QW_ATTN_WAVES * 64, W = D / 8, JT = 256 / D;
+    static constexpr uint32_t KW = T * W / THREADS;        // words of a token that a thread turns
+    static constexpr uint32_t VS = T * D / 16 / THREADS;   // pairs of elements of eight tokens' words
     static constexpr uint32_t K_BYTES = T * D * 2;
 };
 template <int D>
@@ -520,7 +519,7 @@ struct qw_attn_fetch {
 };
 
 template <int DT, int D, bool BIG>
-__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(const qw_attn_args a) {
     typedef qw_attn_tile<D> L;
     constexpr uint32_t T = L::T, W = L::W, JT = L::JT, NT = D / 32, KS = D / 16, HALVES = T / 32;
     __shared__ union __attribute__((aligned(16))) {
@@ -599,25 +598,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void qw_attn_
         u2_t scales = f.v_scale;
         if (t0 + T > s.length) scales = t0 + vt >= s.length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(scales, t0 + vt, s.length);
         far |= qw_attn_far8(scales);
-        if (L::V_THREADS == L::THREADS || tid < L::V_THREADS) {
 #pragma unroll
-            for (uint32_t i = 0; i < L::VS; ++i) {
-                const uint32_t pair = vs + i;
-                uint32_t x[8];
+        for (uint32_t i = 0; i < L::VS; ++i) {
+            const uint32_t pair = vs + i;
+            uint32_t x[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e)
-                    x[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(f.v[e >> 2][e & 3u] >> (8u * pair), qw_attn_unit(scales, e), 0));
-                u4_t even, odd;
+            for (uint32_t e = 0; e < 8; ++e)
+                x[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(f.v[e >> 2][e & 3u] >> (8u * pair), qw_attn_unit(scales, e), 0));
+            u4_t even, odd;
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    even[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
-                    odd[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
-                }
+            for (uint32_t e = 0; e < 4; ++e) {
+                even[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
+                odd[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+            }
 #pragma unroll
-                for (uint32_t o = 0; o < 2; ++o) {
-                    const uint32_t j = 2u * pair + o;
-                    *(u4_t*)(sh.tile.v[slot] + (((j / JT) * (T / 16u) + (vt >> 4)) * 64u + ((vt >> 3) & 1u) * 32u + vw + W * (j % JT)) * 16u) = o ? odd : even;
-                }
+            for (uint32_t o = 0; o < 2; ++o) {
+                const uint32_t j = 2u * pair + o;
+                *(u4_t*)(sh.tile.v[slot] + (((j / JT) * (T / 16u) + (vt >> 4)) * 64u + ((vt >> 3) & 1u) * 32u + vw + W * (j % JT)) * 16u) = o ? odd : even;
             }
         }
     };
@@ -814,34 +811,48 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
-// The kernel of a call and how many parts its rows are split into.  Up to 16 columns (rows x heads of a group) the streaming kernel, else tiles of 128.
-// Parts give a launch that many workgroups (`fill`: one a compute unit for the streaming kernel, whose waves then have steps enough; two rounds and more of
-// what the units hold for the tile kernel), but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more:
-// a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 34 / 38 / 41 us, behind 500 in 1 / 4: 7.0 / 8.5; 64 sequences of up to 8192 in 1 / 2 / 4: 85 / 94 / 98;
-// 2048 rows of a prompt in 1 / 2: 65 / 95; 256 rows behind 16384 in 4 / 7 / 13 / 26: 145 / 158 / 139 / 169; six ragged chunks 1 / 2 / 3: 178 / 163 / 153;
-// windows of 8 rows over 1000 tokens, 32 tiles, in 1 / 2 / 8: 63 / 40 / 25; 16 rows behind 32768, 8 tiles, in 16 / 64 / 128: 59 / 36 / 48.
+// The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds.
+// The streaming kernel turns a token's elements anew for every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for
+// many columns over many tokens, from 256 columns and 2^20 tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128,
+// 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15, 64 of them 78 / 123; 512 rows of a prompt 18 / 21, 1024 35 / 34, 2048 89 / 66, 4096 291 / 196; 256
+// rows behind 16384 142 / 142, 512 258 / 207, behind 4096 72 / 83; heads of 64, 1024 rows 17 / 24, behind 16384 214 / 154, 4096 rows 128 / 95.  With heads of 256, whose tiles
+// leave a compute unit one workgroup, it was the slower one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none.
+// Parts give a launch workgroups enough, but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more.
+// Streaming: one workgroup a compute unit, of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 34 / 38 / 41 us; behind 500 in 1 / 4: 7.0 / 8.5;
+// 64 sequences of up to 8192 in 1 / 2 / 4: 85 / 94 / 98); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024
+// tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 23 / 21 / 24).
+// Tiles: as many as run at once, else three rounds of them, of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 / 207 / 246, 640 in 1 / 2 / 3:
+// 191 / 184 / 201; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 / 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
 struct qw_attn_plan {
     bool stream;
     uint64_t tiles;   // of a sequence and a head
     uint32_t parts;
 };
 static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch* b, uint32_t rows, uint32_t q_heads, uint32_t window) {
-    const uint64_t columns = (uint64_t)(b->max_rows < rows ? b->max_rows : rows) * (q_heads / c->kv_heads);
-    qw_attn_plan p;
-    p.stream = columns <= 16u;
-    p.tiles = p.stream ? 1u : (columns + QW_ATTN_COLUMNS - 1u) / QW_ATTN_COLUMNS;
-    const uint64_t all = p.tiles * c->kv_heads * b->seqs;
+    const uint32_t shared = q_heads / c->kv_heads;
+    const uint64_t columns = (uint64_t)(b->max_rows < rows ? b->max_rows : rows) * shared;
     const uint32_t longest = window && window < b->max_length && b->max_rows < b->max_length - window ? window + b->max_rows : b->max_length;
-    const uint64_t fill = p.stream ? 256u : c->head_dim == 256u ? 512u : c->head_dim == 128u ? 1024u : 2048u;
-    const uint32_t eighth = longest / 8u;   // tokens of a part, at least: few tiles of a short sequence 128
-    const uint32_t least = p.stream ? 128u : all > 256u ? 2048u : eighth < 128u ? 128u : eighth < 512u ? eighth : 512u;
-    p.parts = 1u;
-    if (all < fill && longest > (p.stream ? 1024u : 512u)) {
-        const uint64_t want = (fill + all - 1u) / all;
-        const uint32_t most = (longest + least - 1u) / least;
-        p.parts = want < most ? (uint32_t)want : most;
-        if (p.parts > QW_ATTN_MOST_PARTS) p.parts = QW_ATTN_MOST_PARTS;
+    // workgroups of `width` columns over all sequences, of which ragged ones have fewer than the bound says
+    auto workgroups = [&](uint64_t tiles, uint32_t width) {
+        const uint64_t most = tiles * b->seqs, some = (uint64_t)rows * shared / width + b->seqs;
+        return (most < some ? most : some) * c->kv_heads;
+    };
+    qw_attn_plan p;
+    p.tiles = (columns + QW_ATTN_COLUMNS - 1u) / QW_ATTN_COLUMNS;
+    uint64_t all = workgroups(p.tiles, QW_ATTN_COLUMNS), parts = 1u;
+    p.stream = c->head_dim == 256u || columns < 256u || all * longest < 1u << 20;
+    if (p.stream) {
+        p.tiles = (columns + 15u) / 16u;
+        all = workgroups(p.tiles, 16u);
+        if (longest > (c->head_dim == 256u ? 512u : 1024u)) {
+            parts = std::min<uint64_t>((256u + all - 1u) / all, (longest + 127u) / 128u);
+            if (p.tiles > 1u) parts = std::max(parts, std::min<uint64_t>((1024u + all - 1u) / all, longest / 1024u));
+        }
+    } else {
+        const uint64_t units = c->head_dim == 128u ? 512u : 768u;
+        parts = std::min<uint64_t>(all * 2u <= units ? units / all : 3u * units / all, longest / 1536u);
     }
+    p.parts = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(parts, 1u), QW_ATTN_MOST_PARTS);
     return p;
 }
 static uint64_t qw_attn_part_bytes(uint32_t rows, uint32_t q_heads, uint32_t d) { return (uint64_t)rows * q_heads * (d + 2u) * 4u; }
@@ -872,7 +883,7 @@ static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, bool stream,
     if (stream) {
         if (a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
         else hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
-    } else {
+    } else if constexpr (D != 256) {
         if ((1u << a.geo.page_log2) >= qw_attn_tile<D>::T) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
         else hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
     }
