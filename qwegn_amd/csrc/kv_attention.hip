@@ -60,75 +60,77 @@ __device__ __forceinline__ u2_t qw_attn_tail(u2_t scales, uint32_t t, uint32_t l
     return u2_t{(scales[0] & lo) | (0x7F7F7F7Fu & ~lo), (scales[1] & hi) | (0x7F7F7F7Fu & ~hi)};
 }
 
-// What a lane carries of a step of 32 tokens.  Keys: rows of two 16-row operands, lane (i, g) has elements of token 8 (i / 4) + 4 a + i % 4; values: lane
-// (i, g) has eight elements of each of the tokens 8 g .. 8 g + 7.  A score of operand a, accumulator row 4 g + r, is then token 8 g + 4 a + r: the weights
-// are in place as an operand against the values.
+// What a lane carries of a step of 32 tokens, 16 h .. 16 h + 15 in half h.  Keys: rows of an operand of each half, lane (i, g) has elements of its token i; values: lane
+// (i, g) has eight elements of the tokens 4 g .. 4 g + 3 of both halves.  A score of half h, accumulator row 4 g + r, is then token 16 h + 4 g + r: the weights
+// are in place as an operand against the values, and every load takes whole lines.
 template <int D>
 struct qw_attn_step {
     static constexpr uint32_t SETS = D == 256 ? 2 : 1, WORDS = D == 64 ? 2 : 4;
     uint32_t k[2][SETS][WORDS];
     uint32_t k_scale[2][SETS];
     u4_t v[SETS][2];
-    u2_t v_scale[SETS];
+    uint32_t v_scale[SETS][2];
 };
-// Where a lane's pieces are in a page, from the step's first token on.
+// Where a lane's pieces are in a page, from a half's first token on.
 template <int D>
 struct qw_attn_place {
     uint32_t k, k_scale, v, v_scale;
-    bool k_second, v_second;   // SMALL: of the step's second page
-    template <bool SMALL>
     __device__ __forceinline__ void set(const qw_attn_args& a, uint32_t i, uint32_t g) {
-        const uint32_t kt = 8u * (i >> 2) + (i & 3u), word = D == 64 ? i & 7u : i;
-        k_second = SMALL && i >= 8u, v_second = SMALL && g >= 2u;
-        const uint32_t kp = k_second ? kt - 16u : kt, vp = v_second ? g - 2u : g;
-        k = kp * (D / 2u) + g * (4u * qw_attn_step<D>::WORDS);
-        k_scale = a.geo.k_scales + kp * (D / 32u) + (D == 64 ? g >> 1 : g);
-        v = a.geo.v_codes + (vp * (D / 8u) + word) * 32u;
-        v_scale = a.geo.v_scales + (vp * (D / 32u) + (word >> 2)) * 8u;
+        const uint32_t word = D == 64 ? i & 7u : i;
+        k = i * (D / 2u) + g * (4u * qw_attn_step<D>::WORDS);
+        k_scale = a.geo.k_scales + i * (D / 32u) + (D == 64 ? g >> 1 : g);
+        v = a.geo.v_codes + ((g >> 1) * (D / 8u) + word) * 32u + (g & 1u) * 16u;
+        v_scale = a.geo.v_scales + ((g >> 1) * (D / 32u) + (word >> 2)) * 8u + (g & 1u) * 4u;
     }
 };
-// The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two.  The page is the same for all lanes: scalar loads and addresses.
-template <int D, bool SMALL>
+template <bool ONCE, typename T>
+__device__ __forceinline__ T qw_attn_codes(const T* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+// The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two.  The pages are the same for all lanes: scalar loads and addresses.  ONCE: no other workgroup
+// reads these codes, they pass by the caches.
+template <int D, bool SMALL, bool ONCE>
 __device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t t0, uint32_t length,
                                              const qw_attn_place<D>& at, qw_attn_step<D>& s) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS;
-    const uint32_t in = t0 & ((1u << a.geo.page_log2) - 1u), page0 = (uint32_t)table[t0 >> a.geo.page_log2];
-    const uint8_t* const first = head + (uint64_t)(page0 < a.page_count ? page0 : 0u) * stride;
-    const uint8_t* kp = first;
-    const uint8_t* vp = first;
+    const uint32_t page0 = (uint32_t)table[t0 >> a.geo.page_log2];
+    const uint8_t* piece[2];
+    uint32_t in[2] = {t0 & ((1u << a.geo.page_log2) - 1u), 0u};
+    piece[0] = head + (uint64_t)(page0 < a.page_count ? page0 : 0u) * stride;
     if constexpr (SMALL) {
         const uint32_t page1 = (uint32_t)table[min(t0 + 16u, length - 1u) >> 4];   // a half behind the last token is read from the last page, and masked
-        const uint8_t* const second = head + (uint64_t)(page1 < a.page_count ? page1 : 0u) * stride;
-        kp = at.k_second ? second : first;
-        vp = at.v_second ? second : first;
+        piece[1] = head + (uint64_t)(page1 < a.page_count ? page1 : 0u) * stride;
+    } else {
+        piece[1] = piece[0];
+        in[1] = in[0] + 16u;
     }
-    const uint8_t* const kc = kp + in * (D / 2u);
-    const uint8_t* const ks = kp + in * (D / 32u);
-    const uint8_t* const vc = vp + in * (D / 2u);
-    const uint8_t* const vs = vp + in * (D / 32u);
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h)
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint8_t* const codes = piece[h] + in[h] * (D / 2u);
+        const uint8_t* const scales = piece[h] + in[h] * (D / 32u);
 #pragma unroll
         for (uint32_t c = 0; c < SETS; ++c) {
-            __builtin_memcpy(s.k[h][c], __builtin_assume_aligned(kc + at.k + 4u * h * (D / 2u) + c * 64u, 4 * WORDS), 4 * WORDS);
-            s.k_scale[h][c] = ks[at.k_scale + 4u * h * (D / 32u) + 4u * c];
+            typedef uint32_t words_t __attribute__((ext_vector_type(WORDS)));
+            const words_t k = qw_attn_codes<ONCE>((const words_t*)(codes + at.k + c * 64u));
+            __builtin_memcpy(s.k[h][c], &k, 4 * WORDS);
+            s.k_scale[h][c] = scales[at.k_scale + 4u * c];
+            s.v[c][h] = qw_attn_codes<ONCE>((const u4_t*)(codes + at.v + c * 512u));
+            s.v_scale[c][h] = *(const uint32_t*)(scales + at.v_scale + c * 32u);
         }
-#pragma unroll
-    for (uint32_t c = 0; c < SETS; ++c) {
-        s.v[c][0] = *(const u4_t*)(vc + at.v + c * 512u);
-        s.v[c][1] = *(const u4_t*)(vc + at.v + c * 512u + 16u);
-        s.v_scale[c] = *(const u2_t*)(vs + at.v_scale + c * 32u);
     }
 }
 // Tokens behind the last one: harmless scales.
 template <int D>
 __device__ __forceinline__ void qw_attn_cut(uint32_t t0, uint32_t length, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
 #pragma unroll
-    for (uint32_t c = 0; c < qw_attn_step<D>::SETS; ++c) {
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t t = t0 + 16u * h + 4u * g, there = t + 4u <= length ? ~0u : t >= length ? 0u : (1u << (8u * (length - t))) - 1u;
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
-            if (t0 + 8u * (i >> 2) + (i & 3u) + 4u * h >= length) s.k_scale[h][c] = 127u;
-        s.v_scale[c] = t0 + 8u * g >= length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(s.v_scale[c], t0 + 8u * g, length);
+        for (uint32_t c = 0; c < qw_attn_step<D>::SETS; ++c) {
+            if (t0 + 16u * h + i >= length) s.k_scale[h][c] = 127u;
+            s.v_scale[c][h] = (s.v_scale[c][h] & there) | (0x7F7F7F7Fu & ~there);
+        }
     }
 }
 
@@ -267,7 +269,7 @@ __device__ __forceinline__ float qw_attn_max_rows(float v) {
 
 // The columns c0 .. c0 + 15 over the tokens begin .. end - 1 (begin a multiple of 32).  Whether the range has to be done in the wide form (the same answer in every
 // wave); otherwise its results are written.  All waves of a workgroup call it, the first four work.
-template <int DT, int D, bool SMALL, bool WIDE>
+template <int DT, int D, bool SMALL, bool ONCE, bool WIDE>
 __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_attn_seq& s, uint32_t seq, uint32_t head, uint32_t part, uint32_t c0, uint32_t begin, uint32_t end,
                                                qw_attn_shared<D>& sh) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u;   // ROWS: accumulators, and elements of a column that a thread stores
@@ -296,14 +298,14 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     const uint32_t stride = a.kv_heads * a.geo.piece;
     const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
     qw_attn_place<D> place;
-    place.template set<SMALL>(a, i, g);
+    place.set(a, i, g);
 
     auto one = [&](uint32_t t0, qw_attn_step<D>& now) {
             if (t0 + 32u > s.length) qw_attn_cut<D>(t0, s.length, i, g, now);
             if constexpr (!WIDE) {
 #pragma unroll
                 for (uint32_t c = 0; c < SETS; ++c) {
-                    far |= qw_attn_far8(now.v_scale[c]);
+                    far |= qw_attn_far8(u2_t{now.v_scale[c][0], now.v_scale[c][1]});
                     if constexpr (DT == QWHIP_F16) far |= qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
                     else far_k = max(far_k, max(now.k_scale[0][c], now.k_scale[1][c]));
                 }
@@ -335,7 +337,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                 seen = 0u;
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    const int32_t at = (int32_t)(t0 + 8u * g + e);
+                    const int32_t at = (int32_t)(t0 + 16u * (e >> 2) + 4u * g + (e & 3u));
                     const bool in = at <= pos && at >= low;
                     seen |= in ? 1u << e : 0u;
                     if (!in) x[e >> 2][e & 3u] = -__builtin_inff();
@@ -376,7 +378,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                 u4_t broken = {0, 0, 0, 0};
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    unit[e] = qw_attn_unit(now.v_scale[c], e);
+                    unit[e] = qw_attn_unit(u2_t{now.v_scale[c][0], now.v_scale[c][1]}, e);
                     word[e] = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
                     if constexpr (WIDE) {
                         const bool nan = ((__float_as_uint(unit[e]) >> 23) & 0xFFu) > QW_ATTN_BF16_MOST;
@@ -414,7 +416,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     };
     if (wave < 4u && wave < t.to) {
         // wave w has the steps w, w + 4, ..
-        auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), s.length, place, f); };
+        auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL, ONCE>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), s.length, place, f); };
         qw_attn_step<D> f[WIDE ? 1 : 2];
         if constexpr (WIDE) {
             for (uint32_t step = wave; step < t.to; step += 4u) {
@@ -470,7 +472,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     return false;
 }
 
-template <int DT, int D, bool SMALL>
+template <int DT, int D, bool SMALL, bool ONCE>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
     __shared__ qw_attn_shared<D> sh;
     const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = a.tiles - 1u - rest / a.kv_heads, seq = blockIdx.y;   // the last rows see the most: first
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
     if (tile * 16u >= s.n * a.shared) return;
     const qw_attn_range t = qw_attn_tokens<32>(a, s, tile * 16u, min(tile * 16u + 15u, s.n * a.shared - 1u), part);
     const uint32_t begin = t.first + 32u * t.from, end = t.first + 32u * t.to;
-    if (qw_attn_stream<DT, D, SMALL, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, SMALL, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
+    if (qw_attn_stream<DT, D, SMALL, ONCE, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, SMALL, false, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -724,9 +726,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     if (__syncthreads_or((int)far)) {
         const uint32_t begin = rg.first + rg.from * T, end = rg.first + rg.to * T;
         if (a.geo.page_log2 == 4u)
-            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, true, true>(a, s, seq, head, part, c, begin, end, sh.stream);
+            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, true, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
         else
-            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
+            for (uint32_t c = c0; c < min(c0 + QW_ATTN_COLUMNS, count); c += 16u) qw_attn_stream<DT, D, false, false, true>(a, s, seq, head, part, c, begin, end, sh.stream);
         return;
     }
 
@@ -881,8 +883,11 @@ template <int DT, int D>
 static void qw_launch_attn(qwhip_stream_t s, const qw_attn_args& a, bool stream, uint32_t seqs) {
     const dim3 grid(a.parts * a.kv_heads * a.tiles, seqs);
     if (stream) {
-        if (a.geo.page_log2 == 4u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
-        else hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
+        const bool small = a.geo.page_log2 == 4u;
+        if (a.tiles == 1u && small) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true, true>), grid, dim3(256), 0, s->stream, a);
+        else if (a.tiles == 1u) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false, true>), grid, dim3(256), 0, s->stream, a);
+        else if (small) hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, true, false>), grid, dim3(256), 0, s->stream, a);
+        else hipLaunchKernelGGL((qw_attn_stream_kernel<DT, D, false, false>), grid, dim3(256), 0, s->stream, a);
     } else if constexpr (D != 256) {
         if ((1u << a.geo.page_log2) >= qw_attn_tile<D>::T) hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, true>), grid, dim3(256), 0, s->stream, a);
         else hipLaunchKernelGGL((qw_attn_tile_kernel<DT, D, false>), grid, dim3(256), 0, s->stream, a);
