@@ -251,10 +251,11 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 // Elements become f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves
 // notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
 // two bf16 numbers each, a broken block of values for the rows alone that see its token.
-// Bound by the vector unit (conversions and exchanges of the elements: 96 of some 200 instructions a wave and step) and the bytes: a token of 64 sequences of up to 8192,
-// 40 heads of 128 over 8: 85 us = 4.7 TB/s; a token behind 131077: 34 us (29 and the join), 4.9 TB/s; behind 4096: 8.9 us, latency of two launches.  Steps on
-// the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last step
-// alone, two register sets in turn 85.  The four waves' sums meet in LDS at the end.
+// One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128 over 8: 78 us = 5.2 TB/s of codes and scales (a read of 4 GiB 6.15; the
+// longest sequence's workgroup ends last); behind 131077: 30 us (26 = 5.5 TB/s and the join); behind 4096: 8.9 us, latency of two launches.  Several, which read the same
+// tokens from the L2, by the vector unit (201 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us.
+// Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last
+// step alone, two register sets in turn 85; loads of whole lines, codes as streamed loads 78.  The four waves' sums meet in LDS at the end.
 // ------------------------------------------------------------------------------------------------
 template <int D>
 struct qw_attn_shared {
@@ -484,20 +485,22 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many rows, heads of 64 and 128: four waves of 32 columns each share tiles of 64 tokens.  A tile's codes are on their way while the tile before it is contracted; the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane:
-// a conversion serves all columns of the workgroup.
+// Many rows, heads of 64 and 128: four waves of 32 columns each share tiles of 64 tokens.  A tile's codes are on their way while the tile before it is contracted;
+// the threads then turn them into f16 (keys of bf16 queries: bf16) and leave them in LDS as the operands that the waves read, lane by lane: a conversion serves all
+// columns of the workgroup.
 //   keys     operand of 32 tokens x 16 elements, lane (r, h) elements 8 h .. of token 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4: an accumulator's
 //            scores are then eight tokens in a row, twice, the operand of the weights
 //   values   operand of 32 elements x 16 tokens, lane (r, h) tokens 8 h .. of element 8 (r % W) + j, W = D / 8 words, r / W picking j in its tile
 // A step: the weights of its tile out of its scores, the next tile turned into LDS, a meeting; its values under its weights and the next tile's scores, 32 matrix
 // instructions in a row whose operands come from LDS eight ahead.  One meeting does: what a wave that is ahead turns goes into the half of LDS that all have left
-// behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: some 200 vector
-// instructions a wave and step against 32 matrix ones of 32 cycles), which the two workgroups of a compute unit overlap in part: 4096 rows of a prompt, 40 heads of
-// 128, bf16: 194 us = 885 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six ragged chunks of up to 700 rows behind up to 6001 tokens, 24
-// heads of 64, whose scores cost as much for half the products, in three parts: 152 us = 500 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles
-// through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a wave's priority around them 204; scale bytes four at a time 201; pages and addresses
-// on the scalar unit 194 .. 204 by card; one meeting a step, not two 196.  Eight waves a workgroup turn a tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart
-// leave a SIMD's vector unit to one wave at a time (252); without the wide form behind it the kernel would take 5 % less.
+// behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: 292 vector instructions a wave and step against 32 matrix ones
+// of 32 cycles, which keep that unit busy for 40 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at
+// its full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 192 .. 197 us by card = 895 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230);
+// six ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 150 us =
+// 510 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a
+// wave's priority around them 204; scale bytes four at a time 201; pages and addresses on the scalar unit, one meeting a step 196.  Eight waves a workgroup turn a tile
+// for twice the columns, but meet more of each other (245); two groups of waves half a step apart leave a SIMD's vector unit to one wave at a time (252); without
+// the wide form behind it the kernel would take 5 % less.
 // ------------------------------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
@@ -816,13 +819,13 @@ constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch 
 // The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds.
 // The streaming kernel turns a token's elements anew for every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for
 // many columns over many tokens, from 256 columns and 2^20 tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128,
-// 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15, 64 of them 78 / 123; 512 rows of a prompt 18 / 21, 1024 35 / 34, 2048 89 / 66, 4096 291 / 196; 256
-// rows behind 16384 142 / 142, 512 258 / 207, behind 4096 72 / 83; heads of 64, 1024 rows 17 / 24, behind 16384 214 / 154, 4096 rows 128 / 95.  With heads of 256, whose tiles
+// 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15, 64 of them 78 / 122; 512 rows of a prompt 16 / 21, 1024 33 / 36, 2048 89 / 70, 4096 283 / 217; 256
+// rows behind 16384 142 / 120, 512 259 / 205, behind 4096 70 / 68; heads of 64, 1024 rows 17 / 24, behind 16384 221 / 152, 4096 rows 126 / 93.  With heads of 256, whose tiles
 // leave a compute unit one workgroup, it was the slower one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none.
 // Parts give a launch workgroups enough, but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more.
-// Streaming: one workgroup a compute unit, of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 34 / 38 / 41 us; behind 500 in 1 / 4: 7.0 / 8.5;
-// 64 sequences of up to 8192 in 1 / 2 / 4: 85 / 94 / 98); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024
-// tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 23 / 21 / 24).
+// Streaming: one workgroup a compute unit, of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 32 / 35 / 39 us; behind 500 in 1 / 4: 7.2 / 8.9;
+// 64 sequences of up to 8192 in 1 / 2 / 4: 81 / 83 / 89); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024
+// tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 24 / 21 / 24).
 // Tiles: as many as run at once, else three rounds of them, of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 / 207 / 246, 640 in 1 / 2 / 3:
 // 191 / 184 / 201; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 / 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
 struct qw_attn_plan {
