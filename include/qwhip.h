@@ -626,7 +626,7 @@ qwhip_status qwhip_head_norm_rope(qwhip_stream_t s, const qwhip_head_rules* rule
  *   values' codes   [T / 8][D / 8][8] words of eight elements (lowest element in the lowest nibble), token t at [t / 8][..][t % 8]
  *   values' scales  [T / 8][D / 32][8] bytes
  * (the values' eight tokens side by side are what a lane of the matrix unit contracts).  Scale bytes over 252, which only a block
- * that was not finite gets, read as NaN. */
+ * that was not finite gets, read as NaN; in the attention's products the elements under a scale byte of 0 (below 2^-124) may count as zero. */
 typedef struct qwhip_kv_cache {
     void* pages;         /* device, 16-byte aligned */
     uint64_t bytes;      /* what the caller's region holds from there on */
