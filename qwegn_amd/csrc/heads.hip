@@ -25,13 +25,13 @@ extern "C" qwhip_status qwhip_kv_cache_validate(const qwhip_kv_cache* c) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A head's elements lie eight to a lane: a quad of lanes holds a block of the transform and of the quantiser, 4 to 32 lanes a head.  Every operation is rounded by itself, in a fixed order (the sum is a tree): keys next to a border of the 4-bit grid fall on
-// the side that the definition in fp32 says, from either door and at every number of rows.
-// Bound by the bytes: 8192 rows of 40 + 8 heads of 128, bf16: 39 us = 5.3 TB/s (a copy of 4 GiB 4.8); the same rows with their values into the cache, all of them
-// transformed, codes, scales and values written: 51 us = 4.9 TB/s; one row: the host's call (3.2 .. 3.6 us on the device).  Steps: the rotation's partners loaded and
-// normed a second time 63 us; exchanged between lanes, gammas and table entries once a thread 41; a workgroup has queries, keys or values 39.  Into the cache: a
-// workgroup a row 76 us, whose values' four-byte words went out through eight L2s; eight rows a workgroup 69; the kinds apart, the transform's exchange on its
-// additions 51.
+// A head's elements lie eight to a lane: a quad of lanes holds a block of the transform and of the quantiser, 4 to 32 lanes a head.  Every operation is rounded by
+// itself, in a fixed order (the sum is a tree): keys next to a border of the 4-bit grid fall on the side that the definition in fp32 says, from either door and at
+// every number of rows. Bound by the bytes: 8192 rows of 40 + 8 heads of 128, bf16: 39 us = 5.3 TB/s (a copy of 4 GiB 4.8); the same rows with their values into the
+// cache, all of them transformed, codes, scales and values written: 51 us = 4.9 TB/s; one row: the host's call (3.2 .. 3.6 us on the device).  Steps: the rotation's
+// partners loaded and normed a second time 63 us; exchanged between lanes, gammas and table entries once a thread 41; a workgroup has queries, keys or values 39.
+// Into the cache: a workgroup a row 76 us, whose values' four-byte words went out through eight L2s; eight rows a workgroup 69; the kinds apart, the transform's
+// exchange on its additions 51.
 // ------------------------------------------------------------------------------------------------
 struct qw_heads_side {
     const void* x;

@@ -60,8 +60,8 @@ __device__ __forceinline__ u2_t qw_attn_tail(u2_t scales, uint32_t t, uint32_t l
     return u2_t{(scales[0] & lo) | (0x7F7F7F7Fu & ~lo), (scales[1] & hi) | (0x7F7F7F7Fu & ~hi)};
 }
 
-// What a lane carries of a step of 32 tokens, 16 h .. 16 h + 15 in half h.  Keys: rows of an operand of each half, lane (i, g) has elements of its token i; values: lane
-// (i, g) has eight elements of the tokens 4 g .. 4 g + 3 of both halves.  A score of half h, accumulator row 4 g + r, is then token 16 h + 4 g + r: the weights
+// What a lane carries of a step of 32 tokens, 16 h .. 16 h + 15 in half h.  Keys: rows of an operand of each half, lane (i, g) has elements of its token i; values:
+// lane (i, g) has eight elements of the tokens 4 g .. 4 g + 3 of both halves.  A score of half h, accumulator row 4 g + r, is then token 16 h + 4 g + r: the weights
 // are in place as an operand against the values, and every load takes whole lines.
 template <int D>
 struct qw_attn_step {
@@ -218,8 +218,8 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
     return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
 }
 
-// What a row's sums are multiplied by, and the logarithm of its sum.  A row without a score over -inf has neither.  The largest score's own weight is one, so that a sum
-// of zero under a finite maximum means a scaled score over fp32's range: NaN.
+// What a row's sums are multiplied by, and the logarithm of its sum.  A row without a score over -inf has neither.  The largest score's own weight is one, so that a
+// sum of zero under a finite maximum means a scaled score over fp32's range: NaN.
 __device__ __forceinline__ float qw_attn_inverse(float best, float total) { return best == -__builtin_inff() && total == 0.0f ? 0.0f : 1.0f / total; }
 __device__ __forceinline__ float qw_attn_log(const qw_attn_args& a, float best, float total) {
     return best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
@@ -246,16 +246,16 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 }
 
 // ------------------------------------------------------------------------------------------------
-// Streaming: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on
-// their way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T.
-// Elements become f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves
-// notice at the end of their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as
-// two bf16 numbers each, a broken block of values for the rows alone that see its token.
-// One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128 over 8: 78 us = 5.2 TB/s of codes and scales (a read of 4 GiB 6.15; the
-// longest sequence's workgroup ends last); behind 131077: 30 us (26 = 5.5 TB/s and the join); behind 4096: 8.9 us, latency of two launches.  Several, which read the same
-// tokens from the L2, by the vector unit (201 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us.
-// Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last
-// step alone, two register sets in turn 85; loads of whole lines, codes as streamed loads 78.  The four waves' sums meet in LDS at the end.
+// Streaming: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on their
+// way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T. Elements become
+// f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves notice at the end of
+// their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a
+// broken block of values for the rows alone that see its token. One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128
+// over 8: 78 us = 5.2 TB/s of codes and scales (a read of 4 GiB 6.15; the longest sequence's workgroup ends last); behind 131077: 30 us (26 = 5.5 TB/s and the join);
+// behind 4096: 8.9 us, latency of two launches.  Several, which read the same tokens from the L2, by the vector unit (201 instructions a wave and step, 96 of them
+// turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us. Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four
+// scale bytes at a time 93; pages by scalar loads, the tail's care in the last step alone, two register sets in turn 85; loads of whole lines, codes as streamed
+// loads 78.  The four waves' sums meet in LDS at the end.
 // ------------------------------------------------------------------------------------------------
 template <int D>
 struct qw_attn_shared {
@@ -269,15 +269,17 @@ __device__ __forceinline__ float qw_attn_max_rows(float v) {
 }
 
 // The columns c0 .. c0 + 15 over the tokens begin .. end - 1 (begin a multiple of 32).  Whether the range has to be done in the wide form (the same answer in every
-// wave); otherwise its results are written.  All waves of a workgroup call it, the first four work.
+// wave); otherwise its results are written.  All of a workgroup call it.
 template <int DT, int D, bool SMALL, bool ONCE, bool WIDE>
 __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_attn_seq& s, uint32_t seq, uint32_t head, uint32_t part, uint32_t c0, uint32_t begin, uint32_t end,
                                                qw_attn_shared<D>& sh) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS, ROWS = D / 16u;   // ROWS: accumulators, and elements of a column that a thread stores
     constexpr int VT = WIDE ? QWHIP_BF16 : QWHIP_F16;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), i = lane & 15u, g = lane >> 4, count = s.n * a.shared;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), i = lane & 15u, g = lane >> 4;
+    const uint32_t count = s.n * a.shared;
     qw_attn_range t = qw_attn_tokens<32>(a, s, c0, min(c0 + 15u, count - 1u), 0u);
-    t.first = max(t.first, begin), t.from = 0u, t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
+    t.first = max(t.first, begin), t.from = 0u;
+    t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
     // this lane's column
     const uint32_t col = min(c0 + i, count - 1u), row = col / a.shared, member = col - row * a.shared;
     const int32_t pos = s.pos0 + (int32_t)row, low = (int32_t)qw_attn_low(a, pos);
@@ -302,120 +304,120 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     place.set(a, i, g);
 
     auto one = [&](uint32_t t0, qw_attn_step<D>& now) {
-            if (t0 + 32u > s.length) qw_attn_cut<D>(t0, s.length, i, g, now);
-            if constexpr (!WIDE) {
-#pragma unroll
-                for (uint32_t c = 0; c < SETS; ++c) {
-                    far |= qw_attn_far8(u2_t{now.v_scale[c][0], now.v_scale[c][1]});
-                    if constexpr (DT == QWHIP_F16) far |= qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
-                    else far_k = max(far_k, max(now.k_scale[0][c], now.k_scale[1][c]));
-                }
-            }
-            f4_t x[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                for (uint32_t c = 0; c < SETS; ++c) {
-                    const bool nan = WIDE && now.k_scale[h][c] > QW_ATTN_BF16_MOST;
-                    const float unit = __uint_as_float((nan ? 127u : now.k_scale[h][c]) << 23);
-#pragma unroll
-                    for (uint32_t j = 0; j < WORDS; ++j) {
-                        u4_t k = qw_attn_operand<WIDE ? QWHIP_BF16 : DT>(now.k[h][c][j], unit);
-                        if (nan) k = u4_t{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-                        if constexpr (WIDE && DT == QWHIP_F16) {
-                            u4_t hi, lo, y = q[c][j];
-                            asm volatile("" : "+v"(y));   // split anew every time: the parts would take as many registers again
-                            qw_attn_split(y, hi, lo);
-                            x[h] = qw_attn_mfma<QWHIP_BF16>(k, hi, qw_attn_mfma<QWHIP_BF16>(k, lo, x[h]));
-                        } else {
-                            x[h] = qw_attn_mfma<DT>(k, q[c][j], x[h]);
-                        }
-                    }
-                }
-            // masks where a column does not see the whole step
-            uint32_t seen = 0xFFu;
-            if ((int32_t)(t0 + 31u) > t.pos_a || t0 < t.low_b) {
-                seen = 0u;
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) {
-                    const int32_t at = (int32_t)(t0 + 16u * (e >> 2) + 4u * g + (e & 3u));
-                    const bool in = at <= pos && at >= low;
-                    seen |= in ? 1u << e : 0u;
-                    if (!in) x[e >> 2][e & 3u] = -__builtin_inff();
-                }
-            }
-            const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-            // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
-            if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
-                const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
-                sum *= fade;
-#pragma unroll
-                for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
-                top = larger;
-            }
-            const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
-            float p[8];
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
-            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            u4_t hi, lo, in;   // the weights; wide: as two bf16 numbers, and whether their tokens are seen
-            if constexpr (!WIDE) {
-                h8_t w;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = (h1_t)p[e];
-                hi = __builtin_bit_cast(u4_t, w);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hi[e] = qw_attn_bf16x2(p[2 * e], p[2 * e + 1]);
-                    lo[e] = qw_attn_bf16x2(p[2 * e] - __uint_as_float(hi[e] << 16), p[2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
-                    in[e] = ((seen >> (2 * e)) & 1u ? 0x3F80u : 0u) | ((seen >> (2 * e)) & 2u ? 0x3F800000u : 0u);
-                }
-            }
+        if (t0 + 32u > s.length) qw_attn_cut<D>(t0, s.length, i, g, now);
+        if constexpr (!WIDE) {
 #pragma unroll
             for (uint32_t c = 0; c < SETS; ++c) {
-                float unit[8];
-                uint32_t word[8];
-                u4_t broken = {0, 0, 0, 0};
+                far |= qw_attn_far8(u2_t{now.v_scale[c][0], now.v_scale[c][1]});
+                if constexpr (DT == QWHIP_F16) far |= qw_attn_far<DT>(now.k_scale[0][c]) | qw_attn_far<DT>(now.k_scale[1][c]);
+                else far_k = max(far_k, max(now.k_scale[0][c], now.k_scale[1][c]));
+            }
+        }
+        f4_t x[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) {
-                    unit[e] = qw_attn_unit(u2_t{now.v_scale[c][0], now.v_scale[c][1]}, e);
-                    word[e] = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
-                    if constexpr (WIDE) {
-                        const bool nan = ((__float_as_uint(unit[e]) >> 23) & 0xFFu) > QW_ATTN_BF16_MOST;
-                        unit[e] = nan ? 1.0f : unit[e];
-                        word[e] = nan ? 0u : word[e];
-                        broken[e >> 1] |= nan ? 0x3F80u << (16u * (e & 1u)) : 0u;
+        for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+            for (uint32_t c = 0; c < SETS; ++c) {
+                const bool nan = WIDE && now.k_scale[h][c] > QW_ATTN_BF16_MOST;
+                const float unit = __uint_as_float((nan ? 127u : now.k_scale[h][c]) << 23);
+#pragma unroll
+                for (uint32_t j = 0; j < WORDS; ++j) {
+                    u4_t k = qw_attn_operand<WIDE ? QWHIP_BF16 : DT>(now.k[h][c][j], unit);
+                    if (nan) k = u4_t{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+                    if constexpr (WIDE && DT == QWHIP_F16) {
+                        u4_t hi, lo, y = q[c][j];
+                        asm volatile("" : "+v"(y));   // split anew every time: the parts would take as many registers again
+                        qw_attn_split(y, hi, lo);
+                        x[h] = qw_attn_mfma<QWHIP_BF16>(k, hi, qw_attn_mfma<QWHIP_BF16>(k, lo, x[h]));
+                    } else {
+                        x[h] = qw_attn_mfma<DT>(k, q[c][j], x[h]);
                     }
                 }
-                f4_t bad = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (WIDE) bad = qw_attn_mfma<QWHIP_BF16>(broken, in, bad);   // an accumulator's row is in one block in all of a set's
-                qw_attn_pairs<D == 64 ? 2 : 4>([&](auto pair) {
-                    constexpr int j = decltype(pair)::value;
-                    uint32_t v[8];
-#pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) v[e] = qw_attn_pair<VT, j>(word[e], unit[e]);
-                    u4_t even, odd;
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        even[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05040100u);
-                        odd[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07060302u);
-                    }
-#pragma unroll
-                    for (uint32_t o = 0; o < 2; ++o) {
-                        f4_t& u = acc[8 * c + 2 * j + o];
-                        if constexpr (WIDE) u = qw_attn_mfma<VT>(o ? odd : even, lo, u);
-                        u = qw_attn_mfma<VT>(o ? odd : even, hi, u);
-                        if constexpr (WIDE) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (bad[r] > 0.0f) u[r] = __builtin_nanf("");
-                        }
-                    }
-                });
             }
+        // masks where a column does not see the whole step
+        uint32_t seen = 0xFFu;
+        if ((int32_t)(t0 + 31u) > t.pos_a || t0 < t.low_b) {
+            seen = 0u;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const int32_t at = (int32_t)(t0 + 16u * (e >> 2) + 4u * g + (e & 3u));
+                const bool in = at <= pos && at >= low;
+                seen |= in ? 1u << e : 0u;
+                if (!in) x[e >> 2][e & 3u] = -__builtin_inff();
+            }
+        }
+        const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
+        if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
+            const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
+            sum *= fade;
+#pragma unroll
+            for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
+            top = larger;
+        }
+        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
+        float p[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
+        sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        u4_t hi, lo, in;   // the weights; wide: as two bf16 numbers, and whether their tokens are seen
+        if constexpr (!WIDE) {
+            h8_t w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = (h1_t)p[e];
+            hi = __builtin_bit_cast(u4_t, w);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi[e] = qw_attn_bf16x2(p[2 * e], p[2 * e + 1]);
+                lo[e] = qw_attn_bf16x2(p[2 * e] - __uint_as_float(hi[e] << 16), p[2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
+                in[e] = ((seen >> (2 * e)) & 1u ? 0x3F80u : 0u) | ((seen >> (2 * e)) & 2u ? 0x3F800000u : 0u);
+            }
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < SETS; ++c) {
+            float unit[8];
+            uint32_t word[8];
+            u4_t broken = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                unit[e] = qw_attn_unit(u2_t{now.v_scale[c][0], now.v_scale[c][1]}, e);
+                word[e] = D == 64 ? now.v[c][e >> 2][e & 3u] >> (16u * (i >> 3)) : now.v[c][e >> 2][e & 3u];
+                if constexpr (WIDE) {
+                    const bool nan = ((__float_as_uint(unit[e]) >> 23) & 0xFFu) > QW_ATTN_BF16_MOST;
+                    unit[e] = nan ? 1.0f : unit[e];
+                    word[e] = nan ? 0u : word[e];
+                    broken[e >> 1] |= nan ? 0x3F80u << (16u * (e & 1u)) : 0u;
+                }
+            }
+            f4_t bad = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (WIDE) bad = qw_attn_mfma<QWHIP_BF16>(broken, in, bad);   // an accumulator's row is in one block in all of a set's
+            qw_attn_pairs<D == 64 ? 2 : 4>([&](auto pair) {
+                constexpr int j = decltype(pair)::value;
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) v[e] = qw_attn_pair<VT, j>(word[e], unit[e]);
+                u4_t even, odd;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    even[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05040100u);
+                    odd[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07060302u);
+                }
+#pragma unroll
+                for (uint32_t o = 0; o < 2; ++o) {
+                    f4_t& u = acc[8 * c + 2 * j + o];
+                    if constexpr (WIDE) u = qw_attn_mfma<VT>(o ? odd : even, lo, u);
+                    u = qw_attn_mfma<VT>(o ? odd : even, hi, u);
+                    if constexpr (WIDE) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (bad[r] > 0.0f) u[r] = __builtin_nanf("");
+                    }
+                }
+            });
+        }
     };
-    if (wave < 4u && wave < t.to) {
+    if (wave < t.to) {
         // wave w has the steps w, w + 4, ..
         auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL, ONCE>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), s.length, place, f); };
         qw_attn_step<D> f[WIDE ? 1 : 2];
@@ -442,21 +444,19 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     }
 
     // the four waves' columns, then the columns' rows
-    if (wave < 4u) {
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (g == 0u) sh.stats[wave][i][0] = top, sh.stats[wave][i][1] = sum;
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0u) sh.stats[wave][i][0] = top, sh.stats[wave][i][1] = sum;
 #pragma unroll
-        for (uint32_t j = 0; j < ROWS; ++j)
+    for (uint32_t j = 0; j < ROWS; ++j)
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                const uint32_t m = 4u * g + r;   // the accumulator's row
-                sh.sums[wave][i][D == 64 ? 8u * (m & 7u) + 4u * (m >> 3) + j : 128u * (j >> 3) + 8u * m + (j & 7u)] = acc[j][r];
-            }
-    }
+        for (uint32_t r = 0; r < 4; ++r) {
+            const uint32_t m = 4u * g + r;   // the accumulator's row
+            sh.sums[wave][i][D == 64 ? 8u * (m & 7u) + 4u * (m >> 3) + j : 128u * (j >> 3) + 8u * m + (j & 7u)] = acc[j][r];
+        }
     __syncthreads();
     const uint32_t mine = tid >> 4, at = (tid & 15u) * ROWS;   // 16 threads a column, ROWS elements each
-    if (wave >= 4u || c0 + mine >= count) return false;
+    if (c0 + mine >= count) return false;
     const uint32_t my_row = (c0 + mine) / a.shared, my_head = head * a.shared + (c0 + mine) - my_row * a.shared;
     float best = -__builtin_inff(), total = 0.0f, o[ROWS] = {};
 #pragma unroll
@@ -481,7 +481,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
     if (tile * 16u >= s.n * a.shared) return;
     const qw_attn_range t = qw_attn_tokens<32>(a, s, tile * 16u, min(tile * 16u + 15u, s.n * a.shared - 1u), part);
     const uint32_t begin = t.first + 32u * t.from, end = t.first + 32u * t.to;
-    if (qw_attn_stream<DT, D, SMALL, ONCE, false>(a, s, seq, head, part, tile * 16u, begin, end, sh)) qw_attn_stream<DT, D, SMALL, false, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
+    if (qw_attn_stream<DT, D, SMALL, ONCE, false>(a, s, seq, head, part, tile * 16u, begin, end, sh))
+        qw_attn_stream<DT, D, SMALL, false, true>(a, s, seq, head, part, tile * 16u, begin, end, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -494,13 +495,13 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(c
 // A step: the weights of its tile out of its scores, the next tile turned into LDS, a meeting; its values under its weights and the next tile's scores, 32 matrix
 // instructions in a row whose operands come from LDS eight ahead.  One meeting does: what a wave that is ahead turns goes into the half of LDS that all have left
 // behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: 292 vector instructions a wave and step against 32 matrix ones
-// of 32 cycles, which keep that unit busy for 40 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at
-// its full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 192 .. 197 us by card = 895 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230);
-// six ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 150 us =
-// 510 TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a
-// wave's priority around them 204; scale bytes four at a time 201; pages and addresses on the scalar unit, one meeting a step 196.  Eight waves a workgroup turn a tile
-// for twice the columns, but meet more of each other (245); two groups of waves half a step apart leave a SIMD's vector unit to one wave at a time (252); without
-// the wide form behind it the kernel would take 5 % less.
+// of 32 cycles, which keep that unit busy for 40 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at its
+// full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 192 .. 197 us by card = 895 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six
+// ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 150 us = 510
+// TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a
+// wave's priority around them 204; scale bytes four at a time 201; pages and addresses on the scalar unit, one meeting a step 196.  Eight waves a workgroup turn a
+// tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart leave a SIMD's vector unit to one wave at a time (252);
+// without the wide form behind it the kernel would take 5 % less.
 // ------------------------------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ f16_t qw_attn_mfma32(u4_t a, u4_t b, f16_t c) {
@@ -634,7 +635,10 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
         const uint8_t* const values = sh.tile.v[step & 1u] + lane * 16u;
         const uint8_t* const keys = sh.tile.k[(step + 1u) & 1u] + lane * 16u;
         u4_t y[AHEAD];
-        auto load = [&](int n) { y[n % AHEAD] = n < OUTS ? *(const u4_t*)(values + ((n % NT) * (T / 16u) + n / NT) * 1024u) : *(const u4_t*)(keys + ((n - OUTS) % HALVES * KS + (n - OUTS) / HALVES) * 1024u); };
+        auto load = [&](int n) {
+            y[n % AHEAD] = n < OUTS ? *(const u4_t*)(values + ((n % NT) * (T / 16u) + n / NT) * 1024u)
+                                    : *(const u4_t*)(keys + ((n - OUTS) % HALVES * KS + (n - OUTS) / HALVES) * 1024u);
+        };
 #pragma unroll
         for (uint32_t h = 0; h < HALVES; ++h) x[h] = f16_t{};
 #pragma unroll
@@ -816,18 +820,18 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
-// The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds.
-// The streaming kernel turns a token's elements anew for every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for
-// many columns over many tokens, from 256 columns and 2^20 tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128,
-// 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15, 64 of them 78 / 122; 512 rows of a prompt 16 / 21, 1024 33 / 36, 2048 89 / 70, 4096 283 / 217; 256
-// rows behind 16384 142 / 120, 512 259 / 205, behind 4096 70 / 68; heads of 64, 1024 rows 17 / 24, behind 16384 221 / 152, 4096 rows 126 / 93.  With heads of 256, whose tiles
-// leave a compute unit one workgroup, it was the slower one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none.
-// Parts give a launch workgroups enough, but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more.
-// Streaming: one workgroup a compute unit, of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 32 / 35 / 39 us; behind 500 in 1 / 4: 7.2 / 8.9;
-// 64 sequences of up to 8192 in 1 / 2 / 4: 81 / 83 / 89); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024
-// tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 24 / 21 / 24).
-// Tiles: as many as run at once, else three rounds of them, of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 / 207 / 246, 640 in 1 / 2 / 3:
-// 191 / 184 / 201; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 / 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
+// The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds. The streaming kernel turns a token's elements anew for
+// every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for many columns over many tokens, from 256 columns and 2^20
+// tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128, 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15,
+// 64 of them 78 / 122; 512 rows of a prompt 16 / 21, 1024 33 / 36, 2048 89 / 70, 4096 283 / 217; 256 rows behind 16384 142 / 120, 512 259 / 205, behind 4096 70 / 68;
+// heads of 64, 1024 rows 17 / 24, behind 16384 221 / 152, 4096 rows 126 / 93.  With heads of 256, whose tiles leave a compute unit one workgroup, it was the slower
+// one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none. Parts give a launch workgroups enough, but a
+// part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more. Streaming: one workgroup a compute unit,
+// of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 32 / 35 / 39 us; behind 500 in 1 / 4: 7.2 / 8.9; 64 sequences of up to 8192 in 1 / 2
+// / 4: 81 / 83 / 89); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024 tokens (16 rows behind 32768, 40
+// workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 24 / 21 / 24). Tiles: as many as run at
+// once, else three rounds of them, of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 / 207 / 246, 640 in 1 / 2 / 3: 191 / 184 /
+// 201; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 / 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
 struct qw_attn_plan {
     bool stream;
     uint64_t tiles;   // of a sequence and a head
