@@ -114,9 +114,9 @@ __device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_
             typedef uint32_t words_t __attribute__((ext_vector_type(WORDS)));
             const words_t k = qw_attn_codes<ONCE>((const words_t*)(codes + at.k + c * 64u));
             __builtin_memcpy(s.k[h][c], &k, 4 * WORDS);
-            s.k_scale[h][c] = scales[at.k_scale + 4u * c];
+            s.k_scale[h][c] = qw_attn_codes<ONCE>(scales + at.k_scale + 4u * c);
             s.v[c][h] = qw_attn_codes<ONCE>((const u4_t*)(codes + at.v + c * 512u));
-            s.v_scale[c][h] = *(const uint32_t*)(scales + at.v_scale + c * 32u);
+            s.v_scale[c][h] = qw_attn_codes<ONCE>((const uint32_t*)(scales + at.v_scale + c * 32u));
         }
     }
 }
@@ -247,15 +247,16 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 
 // ------------------------------------------------------------------------------------------------
 // Streaming: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on their
-// way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T. Elements become
-// f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves notice at the end of
-// their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a
-// broken block of values for the rows alone that see its token. One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128
-// over 8: 78 us = 5.2 TB/s of codes and scales (a read of 4 GiB 6.15; the longest sequence's workgroup ends last); behind 131077: 30 us (26 = 5.5 TB/s and the join);
-// behind 4096: 8.9 us, latency of two launches.  Several, which read the same tokens from the L2, by the vector unit (201 instructions a wave and step, 96 of them
-// turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us. Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four
-// scale bytes at a time 93; pages by scalar loads, the tail's care in the last step alone, two register sets in turn 85; loads of whole lines, codes as streamed
-// loads 78.  The four waves' sums meet in LDS at the end.
+// way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T.  Elements become
+// f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves notice at the end of their
+// range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a broken
+// block of values for the rows alone that see its token.
+// One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128 over 8: 73 us = 5.6 TB/s of codes and scales (a read of 4 GiB
+// 6.15); behind 131077: 30 us (25 = 5.7 TB/s and the join); behind 4096: 8.9 us, latency of two launches.  Several, which read the same tokens from the L2, by the
+// vector unit (201 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us.
+// Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last step
+// alone, two register sets in turn 85; loads of whole lines, codes as streamed loads 78; three workgroups a unit, not four: 168 registers, so that the
+// loads of a step stay ahead of it 73 (three steps ahead 75, four 77).  The four waves' sums meet in LDS at the end.
 // ------------------------------------------------------------------------------------------------
 template <int D>
 struct qw_attn_shared {
@@ -474,7 +475,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 }
 
 template <int DT, int D, bool SMALL, bool ONCE>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void qw_attn_stream_kernel(const qw_attn_args a) {
     __shared__ qw_attn_shared<D> sh;
     const uint32_t part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts, head = rest % a.kv_heads, tile = a.tiles - 1u - rest / a.kv_heads, seq = blockIdx.y;   // the last rows see the most: first
     const qw_attn_seq s = qw_attn_sequence(a, seq);
@@ -820,18 +821,21 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
-// The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds. The streaming kernel turns a token's elements anew for
-// every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for many columns over many tokens, from 256 columns and 2^20
-// tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128, 8 rows of 40 columns behind 4096 tokens, one sequence 12 / 15,
-// 64 of them 78 / 122; 512 rows of a prompt 16 / 21, 1024 33 / 36, 2048 89 / 70, 4096 283 / 217; 256 rows behind 16384 142 / 120, 512 259 / 205, behind 4096 70 / 68;
-// heads of 64, 1024 rows 17 / 24, behind 16384 221 / 152, 4096 rows 126 / 93.  With heads of 256, whose tiles leave a compute unit one workgroup, it was the slower
-// one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none. Parts give a launch workgroups enough, but a
-// part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more. Streaming: one workgroup a compute unit,
-// of at least 128 tokens (a token behind 131077 in 16 / 32 / 64 / 128 parts 47 / 32 / 35 / 39 us; behind 500 in 1 / 4: 7.2 / 8.9; 64 sequences of up to 8192 in 1 / 2
-// / 4: 81 / 83 / 89); where several workgroups read the same tokens, bound by the vector unit, four a unit of at least 1024 tokens (16 rows behind 32768, 40
-// workgroups, in 8 / 16 / 32 / 64 parts: 40 / 34 / 33 / 42; 8 sequences of 8 rows behind 4096, 192, in 1 / 2 / 4 / 8: 24 / 24 / 21 / 24). Tiles: as many as run at
-// once, else three rounds of them, of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 / 207 / 246, 640 in 1 / 2 / 3: 191 / 184 /
-// 201; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 / 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
+// The kernel of a call and how many parts its rows are split into, from the shapes and the host's bounds.
+// The streaming kernel turns a token's elements anew for every 16 columns (rows x heads of a group), but has more and shorter workgroups: the tile kernel is for
+// many columns over many tokens, from 256 columns and 2^20 tokens over all its tiles.  Stream / tile, each with the better number of parts, us: heads of 128, 8 rows of
+// 40 columns behind 4096 tokens, one sequence 12 / 15, 64 of them 78 / 122; 512 rows of a prompt 16 / 21, 1024 33 / 36, 2048 89 / 70, 4096 283 / 217; 256 rows behind
+// 16384 142 / 120, 512 259 / 205, behind 4096 70 / 68; heads of 64, 1024 rows 17 / 24, behind 16384 221 / 152, 4096 rows 126 / 93.  With heads of 256, whose tiles leave
+// a compute unit one workgroup, it was the slower one but for 4096 rows of a prompt (271 / 260; 1024 37 / 52; 8 rows in 16 windows of 1000 18 / 25), so it has none.
+// Parts give a launch workgroups enough, but a part has to be worth its share of the join (3 .. 5 us) and of the partial results, which are written and read once more.
+// Streaming: powers of two, so that one part of all heads and tiles meets in one XCD's L2 (8 sequences of 8 rows behind 4096 in 1 / 2 / 3 / 4 / 5 / 8 parts 24 / 23 / 24 /
+// 20 / 23 / 24 us).  A workgroup a range: up to 16 parts two workgroups a compute unit, more for one, of at least 128 tokens (a token behind 131077 in 16 / 32 / 48: 47 / 30 /
+// 33; 4 sequences of up to 32768 in 4 / 8 / 16 / 32: 46 / 29 / 26 / 29; 24 of up to 8192 in 1 / 2 / 4 / 8: 44 / 38 / 35 / 36, 64 of them 74 / 77 / 77 / 84; behind 500 in 1 / 4:
+// 7.2 / 8.9).  Several, bound by the vector unit: 256 workgroups, or 1024 of at least 1024 tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 48: 40 / 33 / 32 /
+// 37; 8 rows behind 4096, 24, in 4 / 8 / 16: 13.0 / 11.4 / 12.5).
+// Tiles: as many as run at once, else two rounds of them (heads of 64: three), of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 /
+// 207 / 246, two chunks of 512 rows, 320, in 1 / 3 / 4: 242 / 199 / 206, eight of up to 256, 640, in 1 / 2: 142 / 152; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 /
+// 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
 struct qw_attn_plan {
     bool stream;
     uint64_t tiles;   // of a sequence and a head
@@ -854,12 +858,16 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
         p.tiles = (columns + 15u) / 16u;
         all = workgroups(p.tiles, 16u);
         if (longest > (c->head_dim == 256u ? 512u : 1024u)) {
-            parts = std::min<uint64_t>((256u + all - 1u) / all, (longest + 127u) / 128u);
-            if (p.tiles > 1u) parts = std::max(parts, std::min<uint64_t>((1024u + all - 1u) / all, longest / 1024u));
+            auto up = [](uint64_t n, uint64_t d) { uint64_t two = 1u; while (two * d < n) two *= 2u; return two; };      // powers of two at or over n / d,
+            auto down = [](uint64_t n, uint64_t d) { uint64_t two = 1u; while (two * 2u * d <= n) two *= 2u; return two; };   // at or under it (one at least)
+            if (p.tiles == 1u) parts = up(512u, all) <= 16u ? up(512u, all) : std::max<uint64_t>(16u, up(256u, all));
+            else parts = down(342u, all);
+            parts = std::min(parts, down(longest, 128u));
+            if (p.tiles > 1u) parts = std::max(parts, std::min(up(1024u, all), down(longest, 1024u)));
         }
     } else {
-        const uint64_t units = c->head_dim == 128u ? 512u : 768u;
-        parts = std::min<uint64_t>(all * 2u <= units ? units / all : 3u * units / all, longest / 1536u);
+        const uint64_t units = c->head_dim == 128u ? 512u : 768u, rounds = c->head_dim == 128u ? 2u : 3u;
+        parts = std::min<uint64_t>(all * 2u <= units ? units / all : rounds * units / all, longest / 1536u);
     }
     p.parts = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(parts, 1u), QW_ATTN_MOST_PARTS);
     return p;
