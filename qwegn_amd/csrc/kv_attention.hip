@@ -252,7 +252,7 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 // range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a broken
 // block of values for the rows alone that see its token.
 // One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128 over 8: 73 us = 5.6 TB/s of codes and scales (a read of 4 GiB
-// 6.15); behind 131077: 30 us (25 = 5.7 TB/s and the join); behind 4096: 8.9 us, latency of two launches.  Several, which read the same tokens from the L2, by the
+// 6.15); behind 131077: 30 us (26 = 5.5 TB/s and the join); behind 4096: 8.7 us, latency of two launches.  Several, which read the same tokens from the L2, by the
 // vector unit (201 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us.
 // Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last step
 // alone, two register sets in turn 85; loads of whole lines, codes as streamed loads 78; three workgroups a unit, not four: 168 registers, so that the
