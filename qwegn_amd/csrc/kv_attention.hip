@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void qw_attn_
 // behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: 292 vector instructions a wave and step against 32 matrix ones
 // of 32 cycles, which keep that unit busy for 40 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at its
 // full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 192 .. 197 us by card = 895 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six
-// ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 150 us = 510
+// ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 154 us = 510
 // TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a
 // wave's priority around them 204; scale bytes four at a time 201; pages and addresses on the scalar unit, one meeting a step 196.  Eight waves a workgroup turn a
 // tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart leave a SIMD's vector unit to one wave at a time (252);
@@ -858,8 +858,16 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
         p.tiles = (columns + 15u) / 16u;
         all = workgroups(p.tiles, 16u);
         if (longest > (c->head_dim == 256u ? 512u : 1024u)) {
-            auto up = [](uint64_t n, uint64_t d) { uint64_t two = 1u; while (two * d < n) two *= 2u; return two; };      // powers of two at or over n / d,
-            auto down = [](uint64_t n, uint64_t d) { uint64_t two = 1u; while (two * 2u * d <= n) two *= 2u; return two; };   // at or under it (one at least)
+            auto up = [](uint64_t n, uint64_t d) {   // the power of two at or over n / d
+                uint64_t two = 1u;
+                while (two * d < n) two *= 2u;
+                return two;
+            };
+            auto down = [](uint64_t n, uint64_t d) {   // at or under it, one at least
+                uint64_t two = 1u;
+                while (two * 2u * d <= n) two *= 2u;
+                return two;
+            };
             if (p.tiles == 1u) parts = up(512u, all) <= 16u ? up(512u, all) : std::max<uint64_t>(16u, up(256u, all));
             else parts = down(342u, all);
             parts = std::min(parts, down(longest, 128u));
