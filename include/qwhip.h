@@ -667,8 +667,8 @@ typedef struct qwhip_kv_batch {
 /* out [rows, q_heads, head_dim] = softmax(scale q . K^T) V over the tokens at or before a row's position, and behind position - window
  * with a window (0: none).  q and out f16 or bf16 (pitches ld_q, ld_out elements, 0 = tight; rows 16-byte aligned), query head h with
  * key head h / (q_heads / kv_heads); q_heads <= 65535, a sequence's rows * q_heads up to 2^26; 0 < scale < 2^127.  lse (may be NULL): f32
- * [rows, q_heads], the logarithm of the sum.  A row that sees no token, or only scores of -inf, gets zeros and lse = -inf, one with a scaled score over
- * fp32's range NaN; rows behind the last sequence's are left as they were.  A token that a row does not see does not reach it, whatever its page
+ * [rows, q_heads], the logarithm of the sum.  A row that sees no token, or only scaled scores of -inf (ones under fp32's range among them), gets zeros and
+ * lse = -inf, one with a scaled score over fp32's range NaN, whatever the rows and heads beside it have; rows behind the last sequence's are left as they were.  A token that a row does not see does not reach it, whatever its page
  * holds (NaN among it).
  * fp32 softmax and sums of exact products with q; a weight is rounded to f16 in front of the product with the values.  Out overlaps
  * neither q nor the cache.

@@ -12,10 +12,10 @@ struct qw_attn_args {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    float* part;           // [parts][rows][q_heads][D] sums, then [parts][rows][q_heads][2] maximum (of raw scores) and sum of weights
+    float* part;           // [parts][rows][q_heads][D] sums, then [parts][rows][q_heads][2] maximum (of scaled scores, in binary digits) and sum of weights
     qw_kv_geometry geo;
     uint32_t page_count, kv_heads, ld_table, max_rows, max_length, rows, q_heads, shared, ld_q, ld_out, window, parts, tiles;
-    float scale, scale2;   // scale2 = scale * log2(e)
+    float scale2;          // scale * log2(e)
 };
 
 // A sequence's rows and tokens, cut to what the host allows; the position of its first row.
@@ -218,11 +218,13 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
     return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
 }
 
-// What a row's sums are multiplied by, and the logarithm of its sum.  A row without a score over -inf has neither.  The largest score's own weight is one, so that a
-// sum of zero under a finite maximum means a scaled score over fp32's range: NaN.
+// What a row's sums are multiplied by, and the logarithm of its sum.  Maxima are of scaled scores: one under fp32's range is -inf and none at all, and a row
+// without a score over -inf has neither; one over the range is an infinity under which nothing has a finite weight: NaN.  The sum's exponent goes to the maximum
+// first, so that the logarithm of what is left has all of its bits.
 __device__ __forceinline__ float qw_attn_inverse(float best, float total) { return best == -__builtin_inff() && total == 0.0f ? 0.0f : 1.0f / total; }
-__device__ __forceinline__ float qw_attn_log(const qw_attn_args& a, float best, float total) {
-    return best == -__builtin_inff() && total == 0.0f ? -__builtin_inff() : best * a.scale + 0.6931471805599453f * __builtin_amdgcn_logf(total);
+__device__ __forceinline__ float qw_attn_log(float best, float total) {
+    if (best == -__builtin_inff() && total == 0.0f) return -__builtin_inff();
+    return 0.6931471805599453f * ((best + (float)__builtin_amdgcn_frexp_expf(total)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(total)));
 }
 
 // E elements from `at` on of a row and head: into the output where the range is the whole, else with the range's maximum and sum into the workspace.
@@ -242,7 +244,7 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
     for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
 #pragma unroll
     for (uint32_t e = 0; e < E; e += E < 8u ? E : 8u) qw_attn_store<DT, (E < 8u ? E : 8u)>(y + e, o + e);
-    if (a.lse && first) a.lse[item] = qw_attn_log(a, best, total);
+    if (a.lse && first) a.lse[item] = qw_attn_log(best, total);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -296,7 +298,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     f4_t acc[ROWS];
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of raw scores
+    float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of scaled scores
     uint32_t far = 0, far_k = 0;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
@@ -347,16 +349,16 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
                 if (!in) x[e >> 2][e & 3u] = -__builtin_inff();
             }
         }
-        const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))) * a.scale2;
         // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
-        if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
-            const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
+        if (__ballot(most > top + 8.0f) != 0ull) {
+            const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top - (larger == -__builtin_inff() ? 0.0f : larger));
             sum *= fade;
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
             top = larger;
         }
-        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
+        const float shift = top == -__builtin_inff() ? 0.0f : top;
         float p[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
@@ -462,10 +464,10 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     float best = -__builtin_inff(), total = 0.0f, o[ROWS] = {};
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) best = fmaxf(best, sh.stats[w][mine][0]);
-    const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale2;
+    const float shift = best == -__builtin_inff() ? 0.0f : best;
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(sh.stats[w][mine][0] * a.scale2 - shift);
+        const float f = __builtin_amdgcn_exp2f(sh.stats[w][mine][0] - shift);
         total += f * sh.stats[w][mine][1];
 #pragma unroll
         for (uint32_t e = 0; e < ROWS; ++e) o[e] += f * sh.sums[w][mine][at + e];
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     f16_t acc[NT];
 #pragma unroll
     for (uint32_t j = 0; j < NT; ++j) acc[j] = f16_t{};
-    float top = -__builtin_inff(), sum = 0.0f;   // top: the running maximum that the weights stand under, of raw scores
+    float top = -__builtin_inff(), sum = 0.0f;   // top: the running maximum that the weights stand under, of scaled scores
 
     // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
     const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
@@ -675,16 +677,17 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
         for (uint32_t h = 0; h < HALVES; ++h)
 #pragma unroll
             for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, x[h][e]);
+        most *= a.scale2;
         // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
-        if (__ballot(most * a.scale2 > top * a.scale2 + 8.0f) != 0ull) {
+        if (__ballot(most > top + 8.0f) != 0ull) {
             const float larger = fmaxf(top, fmaxf(most, __shfl_xor(most, 32, 64)));
-            const float fade = __builtin_amdgcn_exp2f(top * a.scale2 - (larger == -__builtin_inff() ? 0.0f : larger * a.scale2));
+            const float fade = __builtin_amdgcn_exp2f(top - (larger == -__builtin_inff() ? 0.0f : larger));
             sum *= fade;
 #pragma unroll
             for (uint32_t j = 0; j < NT; ++j) acc[j] = acc[j] * fade;
             top = larger;
         }
-        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale2;
+        const float shift = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
         for (uint32_t h = 0; h < HALVES; ++h) {
 #pragma unroll
@@ -782,11 +785,11 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
         }
 #pragma unroll
         for (uint32_t p = 0; p < QW_ATTN_FEW_PARTS; ++p) best = fmaxf(best, st[p][0]);
-        const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale2;
+        const float shift = best == -__builtin_inff() ? 0.0f : best;
 #pragma unroll
         for (uint32_t p = 0; p < QW_ATTN_FEW_PARTS; ++p) {
             if (p >= a.parts) break;
-            const float f = __builtin_amdgcn_exp2f(st[p][0] * a.scale2 - shift);
+            const float f = __builtin_amdgcn_exp2f(st[p][0] - shift);
             total += f * st[p][1];
             o += f * y[p];
         }
@@ -798,7 +801,7 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
         if ((tid & 63u) == 0u) fold[0][tid >> 6] = best;
         __syncthreads();
         best = fmaxf(fmaxf(fold[0][0], fold[0][1]), fmaxf(fold[0][2], fold[0][3]));
-        const float f = __builtin_amdgcn_exp2f(st[0] * a.scale2 - (best == -__builtin_inff() ? 0.0f : best * a.scale2));
+        const float f = __builtin_amdgcn_exp2f(st[0] - (best == -__builtin_inff() ? 0.0f : best));
         weight[tid] = f;
         total = f * st[1];
 #pragma unroll
@@ -817,7 +820,7 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
     const float inv = qw_attn_inverse(best, total);
     float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     qw_attn_store<DT, 4>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * 4u, y);
-    if (a.lse && tid % LANES == 0u) a.lse[item] = qw_attn_log(a, best, total);
+    if (a.lse && tid % LANES == 0u) a.lse[item] = qw_attn_log(best, total);
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
@@ -952,7 +955,7 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     a.page_count = cache->page_count, a.kv_heads = cache->kv_heads, a.ld_table = batch->ld_table, a.max_rows = max_rows, a.max_length = batch->max_length;
     a.rows = rows, a.q_heads = q_heads, a.shared = shared, a.ld_q = ld_q, a.ld_out = ld_out, a.window = window > 0x7FFFFFFFu ? 0u : window;
     a.tiles = (uint32_t)plan.tiles;
-    a.scale = scale, a.scale2 = scale * 1.4426950408889634f;
+    a.scale2 = scale * 1.4426950408889634f;
     a.parts = 1;
     if (workspace) {
         a.parts = plan.parts;

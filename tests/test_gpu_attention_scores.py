@@ -1,0 +1,65 @@
+"""qwhip_kv_attention_mxfp4 at the ends of what scores and weights can be, in the streaming and in the tile kernel: small weights beside a large one, scaled scores under
+fp32's range and far from zero, values near fp32's range.
+
+Bounds: half a step of the output's type, half a step of f16 (2^-11) of each weight, e = (D + 8) 2^-24 scale sum |q k| + 2^-20 of a score.  Where a weight
+is subnormal in f16 half of that type's smallest step, 2^-25: weights stand at 2^12 and more under the maximum, so n of them are off by n 2^-37 max |v| of the sum."""
+import numpy as np
+import pytest
+
+from oracle import qwkv
+from qwegn_amd import qwhip
+from tests.test_gpu_attention import HALF_STEP, Case
+from tests.test_gpu_attention_tiles import Tiles
+from tests.test_gpu_heads import decode, encode
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return qwhip.Device(0)
+
+
+def fill(c, seq, k, v):
+    """Keys and values [n, heads, d] as the tokens of a sequence."""
+    t = np.arange(len(k))
+    c.cache.put(c.table[seq][t // c.page] * c.page + t % c.page, np.asarray(k, np.float32), np.asarray(v, np.float32))
+
+
+ROWS = [(Case, [1], 0), (Case, [1], 1 << 24), (Case, [9], 1 << 24), (Tiles, [64], 0), (Tiles, [64], 1 << 24)]
+
+
+@pytest.mark.parametrize("cls,rows,room", ROWS)
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_scaled_scores_under_the_range(dev, cls, rows, room, t):
+    """Rows whose scaled scores are all under fp32's range have only scores of -inf: zeros and -inf, whatever the rows beside them have.  Rows with some of them
+    have the others alone, rows with one over the range NaN."""
+    n, d, scale = 3000, 64, 1.6e38
+    c = cls(dev, 2, d, 1, 4, 32, rows, [n], t, scale=scale, noise=False)
+    k = np.ones((n, 1, d))
+    k[1::3] = 0.0
+    v = np.random.default_rng(3).standard_normal((n, 1, d))
+    fill(c, 0, k, v)
+    q = np.zeros((c.total, 4, d))
+    q[:, 0], q[:, 3] = -1.0, 0.0                                                          # zeros of the second kind: -64 1.6e38 or 0
+    if rows[0] > 1:
+        q[1:rows[0]:2, 3] = 1.0                                                           # over the range
+    c.q = encode(q, t)
+    half = np.ones((n, 1, d))                                                             # and once without a token of score zero
+    for keys, low in ((k, False), (half, True)):
+        fill(c, 0, keys, v)
+        y, l = c.run(room=room)
+        got = decode(y[: rows[0]], t).astype(np.float64)
+        kk, vv = c.cache.tokens(c.table[0], n)
+        for i in range(rows[0]):
+            seen = n - rows[0] + i + 1
+            for h in range(4):
+                if q[i, h, 0] > 0:
+                    assert np.isnan(got[i, h]).all() and np.isnan(l[i, h]), (i, h)
+                elif q[i, h, 0] < 0 and low:
+                    assert (got[i, h] == 0).all() and l[i, h] == -np.inf, (i, h)
+                else:
+                    own = np.arange(seen) % 3 == 1 if q[i, h, 0] < 0 else np.arange(seen) >= 0
+                    x = vv[0, :seen][own]
+                    tol = HALF_STEP[t] * np.abs(x.mean(0)) + 2.0 ** -11 * 1.01 * np.abs(x).mean(0) + 2.0 ** -25
+                    assert (np.abs(got[i, h] - x.mean(0)) <= tol).all() and abs(l[i, h] - np.log(len(x))) <= 2.0 ** -18, (i, h)
