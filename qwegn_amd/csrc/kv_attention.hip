@@ -218,6 +218,12 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
     return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
 }
 
+// A weight's exponent is one multiply-add of the product q.k, which is not rounded in between, but `top` comes from a rounded score: all weights of a column are off by the
+// power of that rounding.  It cancels, but from 2^23 binary digits on it takes weights out of any range.  A range with such a column, from 2^17 on, is done in the wide
+// form, which rounds a score before it takes `top` off: the largest weight is one whatever the score.  (Both ways in a step cost every call one percent.)
+constexpr float QW_ATTN_FAR_SCORE = 0x1p17f;
+__device__ __forceinline__ uint32_t qw_attn_far_score(float top) { return fabsf(top) >= QW_ATTN_FAR_SCORE && top != -__builtin_inff() ? 1u : 0u; }
+
 // What a row's sums are multiplied by, and the logarithm of its sum.  Maxima are of scaled scores: one under fp32's range is -inf and none at all, and a row
 // without a score over -inf has neither; one over the range is an infinity under which nothing has a finite weight: NaN.  The sum's exponent goes to the maximum
 // first, so that the logarithm of what is left has all of its bits.
@@ -357,11 +363,12 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
             top = larger;
+            if constexpr (!WIDE) far |= qw_attn_far_score(top);
         }
         const float shift = top == -__builtin_inff() ? 0.0f : top;
         float p[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
+        for (uint32_t e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(WIDE ? x[e >> 2][e & 3u] * a.scale2 - shift : __builtin_fmaf(x[e >> 2][e & 3u], a.scale2, -shift));
         sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         u4_t hi, lo, in;   // the weights; wide: as two bf16 numbers, and whether their tokens are seen
         if constexpr (!WIDE) {
@@ -686,6 +693,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
 #pragma unroll
             for (uint32_t j = 0; j < NT; ++j) acc[j] = acc[j] * fade;
             top = larger;
+            far |= qw_attn_far_score(top);
         }
         const float shift = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll

@@ -63,3 +63,34 @@ def test_scaled_scores_under_the_range(dev, cls, rows, room, t):
                     x = vv[0, :seen][own]
                     tol = HALF_STEP[t] * np.abs(x.mean(0)) + 2.0 ** -11 * 1.01 * np.abs(x).mean(0) + 2.0 ** -25
                     assert (np.abs(got[i, h] - x.mean(0)) <= tol).all() and abs(l[i, h] - np.log(len(x))) <= 2.0 ** -18, (i, h)
+
+
+@pytest.mark.parametrize("cls,rows,room", ROWS)
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [2.0 ** 14, 2.0 ** 20 + 3.0, 1e8, 1e9, 3e12, 1e30])
+def test_scores_far_from_zero(dev, cls, rows, room, t, scale):
+    """Scaled scores of 2^14 .. 2^110, distinct ones far apart: a row's largest tokens share all of the weight, equal ones equally, and fp32's rounding of a score far
+    from zero is no factor of the weight.  The products are exact in fp32 here, so that equal is equal."""
+    n, d, heads, shared = 1900, 64, 2, 4
+    c = cls(dev, 4, d, heads, shared, 16, rows, [n], t, scale=scale, noise=False)
+    rng = np.random.default_rng(5)
+    k = rng.standard_normal((n, heads, d))
+    k = k[np.arange(n) % 41]                                                              # every key 46 times
+    k[:, 1] = k[0, 1]                                                                     # the second head: one score, far over or under zero
+    fill(c, 0, k, rng.standard_normal((n, heads, d)))
+    q = rng.integers(-7, 8, (c.total, heads * shared, d)).astype(np.float64)
+    c.q = encode(q, t)
+    y, l = c.run(room=room)
+    kk, vv = c.cache.tokens(c.table[0], n)
+    for i in range(rows[0]):
+        for h in range(heads * shared):
+            seen = n - rows[0] + i + 1
+            x = kk[h // shared, :seen] @ q[i, h]
+            assert (x * 64 == np.round(x * 64)).all() and np.abs(kk[h // shared, 0]) @ np.abs(q[i, h]) < 2.0 ** 15   # exact in fp32
+            best = x == x.max()
+            assert best.all() or (x.max() - x[~best].max()) * scale > 200.0
+            v = vv[h // shared, :seen][best]
+            want, size, lse = v.mean(0), np.abs(v).mean(0), x.max() * scale + np.log(len(v))
+            off = np.abs(decode(y[i, h], t).astype(np.float64) - want)
+            assert (off <= HALF_STEP[t] * np.abs(want) + 2.0 ** -11 * 1.01 * size + 2.0 ** -25).all(), (i, h, x.max())
+            assert abs(l[i, h] - lse) <= 2.0 ** -21 * abs(lse) + 2.0 ** -18, (i, h)
