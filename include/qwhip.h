@@ -670,8 +670,8 @@ typedef struct qwhip_kv_batch {
  * [rows, q_heads], the logarithm of the sum.  A row that sees no token, or only scaled scores of -inf (ones under fp32's range among them), gets zeros and
  * lse = -inf, one with a scaled score over fp32's range NaN, whatever the rows and heads beside it have; rows behind the last sequence's are left as they were.  A token that a row does not see does not reach it, whatever its page
  * holds (NaN among it).
- * fp32 softmax and sums of exact products with q; a weight is rounded to f16 in front of the product with the values.  Out overlaps
- * neither q nor the cache.
+ * fp32 softmax and sums of exact products with q; a weight is rounded to f16 in front of the product with the values: to 11 bits down to
+ * 2^-26 of the row's largest, to steps of 2^-36 of that below.  Out overlaps neither q nor the cache.
  * workspace (may be NULL; 16-byte aligned): lets few rows over long sequences split these over more compute units, partial results
  * are joined in a fixed order; at most qwhip_kv_attention_workspace_bytes(..) bytes are used, less room gives fewer parts.  The parts follow
  * from the shapes, the bounds and the room, so a row's bits may depend on them.  Two calls that overlap in time take two workspaces. */

@@ -12,7 +12,7 @@ struct qw_attn_args {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    float* part;           // [parts][rows][q_heads][D] sums, then [parts][rows][q_heads][2] maximum (of scaled scores, in binary digits) and sum of weights
+    float* part;           // [parts][rows][q_heads][D] sums, then [parts][rows][q_heads][2] what the weights' exponents are less (`top`) and the sum of weights
     qw_kv_geometry geo;
     uint32_t page_count, kv_heads, ld_table, max_rows, max_length, rows, q_heads, shared, ld_q, ld_out, window, parts, tiles;
     float scale2;          // scale * log2(e)
@@ -218,9 +218,17 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
     return __uint_as_float((e & 3u) == 3u ? w >> 1 : w << (23u - 8u * (e & 3u)));
 }
 
+// A weight is 2 to the power of its scaled score (in binary digits) less `top`: the column's maximum less QW_ATTN_UNDER when it was last taken.  A maximum that grows is taken
+// again only where a weight would pass 2^QW_ATTN_ROOM, so that sums and accumulators are hardly ever scaled.  f16 holds up to 2^15.999, 11 bits from 2^-14 on and steps
+// of 2^-24 below: weights from 2^-26 of the largest on have all their bits, n smaller ones are off by n 2^-37 of it.  (Weights of at most one would be lost to the values
+// from 2^-25 on, and stay in the sum.)  Room for a growth of 3.9 digits costs 0 .. 1.5 % over room for 8, 3 digits 2 .. 3 % (a prompt of 4096 rows 195.6, 194.4,
+// 199.3 us).  The wide form's bf16 numbers have fp32's range.
+constexpr float QW_ATTN_UNDER = 12.0f, QW_ATTN_ROOM = 15.9f, QW_ATTN_ROOM_WIDE = 8.0f;
+
 // A weight's exponent is one multiply-add of the product q.k, which is not rounded in between, but `top` comes from a rounded score: all weights of a column are off by the
-// power of that rounding.  It cancels, but from 2^23 binary digits on it takes weights out of any range.  A range with such a column, from 2^17 on, is done in the wide
-// form, which rounds a score before it takes `top` off: the largest weight is one whatever the score.  (Both ways in a step cost every call one percent.)
+// power of that rounding.  It cancels, but from 2^23 binary digits on it takes weights out of any range.  A range with such a column, from 2^17 on (under it
+// the rounding is within the tenth of a digit that the room leaves), is done in the wide form, which rounds a score before it takes `top` off: the largest weight is one
+// whatever the score.  (Both ways in a step cost every call one percent.)
 constexpr float QW_ATTN_FAR_SCORE = 0x1p17f;
 __device__ __forceinline__ uint32_t qw_attn_far_score(float top) { return fabsf(top) >= QW_ATTN_FAR_SCORE && top != -__builtin_inff() ? 1u : 0u; }
 
@@ -304,7 +312,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     f4_t acc[ROWS];
 #pragma unroll
     for (uint32_t j = 0; j < ROWS; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float top = -__builtin_inff(), sum = 0.0f;   // top: the maximum that the weights stand under, of scaled scores
+    float top = -__builtin_inff(), sum = 0.0f;   // top: what the weights' exponents are less
     uint32_t far = 0, far_k = 0;
     const uint8_t* const pages = a.pages + (uint64_t)head * a.geo.piece;
     const uint32_t stride = a.kv_heads * a.geo.piece;
@@ -356,9 +364,10 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
             }
         }
         const float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))) * a.scale2;
-        // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
-        if (__ballot(most > top + 8.0f) != 0ull) {
-            const float larger = fmaxf(top, qw_attn_max_rows(most)), fade = __builtin_amdgcn_exp2f(top - (larger == -__builtin_inff() ? 0.0f : larger));
+        // where no weight is too large lanes need not meet (the first score always is)
+        if (__ballot(most - top > (WIDE ? QW_ATTN_ROOM_WIDE : QW_ATTN_ROOM)) != 0ull) {
+            const float all = qw_attn_max_rows(most), larger = all - top > (WIDE ? QW_ATTN_ROOM_WIDE : QW_ATTN_ROOM) ? all - (WIDE ? 0.0f : QW_ATTN_UNDER) : top;
+            const float fade = __builtin_amdgcn_exp2f(top - (larger == -__builtin_inff() ? 0.0f : larger));
             sum *= fade;
 #pragma unroll
             for (uint32_t j = 0; j < ROWS; ++j) acc[j] = acc[j] * fade;
@@ -566,7 +575,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     f16_t acc[NT];
 #pragma unroll
     for (uint32_t j = 0; j < NT; ++j) acc[j] = f16_t{};
-    float top = -__builtin_inff(), sum = 0.0f;   // top: the running maximum that the weights stand under, of scaled scores
+    float top = -__builtin_inff(), sum = 0.0f;   // top: what the weights' exponents are less
 
     // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
     const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
@@ -685,9 +694,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
 #pragma unroll
             for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, x[h][e]);
         most *= a.scale2;
-        // a maximum that grew by less than 8 binary digits stays: weights up to 256, and lanes need not meet (the first one always grows)
-        if (__ballot(most > top + 8.0f) != 0ull) {
-            const float larger = fmaxf(top, fmaxf(most, __shfl_xor(most, 32, 64)));
+        // where no weight is too large lanes need not meet (the first score always is)
+        if (__ballot(most - top > QW_ATTN_ROOM) != 0ull) {
+            const float all = fmaxf(most, __shfl_xor(most, 32, 64)), larger = all - top > QW_ATTN_ROOM ? all - QW_ATTN_UNDER : top;
             const float fade = __builtin_amdgcn_exp2f(top - (larger == -__builtin_inff() ? 0.0f : larger));
             sum *= fade;
 #pragma unroll

@@ -29,6 +29,28 @@ def fill(c, seq, k, v):
 ROWS = [(Case, [1], 0), (Case, [1], 1 << 24), (Case, [9], 1 << 24), (Tiles, [64], 0), (Tiles, [64], 1 << 24)]
 
 
+@pytest.mark.parametrize("cls,rows,room,d", [(*r, d) for r in ROWS for d in (64, 128, 256) if r[0] is Case or d < 256])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_a_long_tail_behind_sinks_of_no_value(dev, cls, rows, room, d, t):
+    """Four tokens whose values are zero hold nearly all of the weight, 16000 others lie 14, 16, 18 and 20 nats (up to 29 binary digits) below: the output is theirs."""
+    n, rng = 16300, np.random.default_rng(d)
+    c = cls(dev, 1, d, 1, 4, 64, rows, [n], t, scale=8.0 / d, noise=False)
+    k, v = np.zeros((n, 1, d)), rng.uniform(0.5, 1.5, (n, 1, d))
+    k[[0, 32, 64, 96]], v[[0, 32, 64, 96]] = 1.0, 0.0                                     # one for each of four ranges that interleave
+    fill(c, 0, k, v)
+    q = np.broadcast_to(np.array([1.75, 2.0, 2.25, 2.5])[None, :, None], (c.total, 4, d))
+    c.q = encode(q, t)
+    y, l = c.run(room=room)
+    kk, vv = c.cache.tokens(c.table[0], n)
+    want, lse, size = qwkv.attention(q[: rows[0]], kk, vv, 8.0 / d)
+    e = (d + 8) * 2.0 ** -24 * 20.0 + 2.0 ** -20
+    assert (want[:, 3].max() < 2.0 ** -11)                                                # what is there to be lost
+    tol = HALF_STEP[t] * np.abs(want) + (2.0 ** -11 * 1.01 + 2 * e) * size + n * 2.0 ** -37 * vv.max() + 2.0 ** -25 * (t == "f16")
+    off = np.abs(decode(y[: rows[0]], t).astype(np.float64) - want)
+    assert (off <= tol).all(), (np.max(off / tol), np.max(off / want))
+    assert (np.abs(l[: rows[0]] - lse) <= e + 2.0 ** -22 * (np.abs(lse) + np.log(n))).all()
+
+
 @pytest.mark.parametrize("cls,rows,room", ROWS)
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 def test_scaled_scores_under_the_range(dev, cls, rows, room, t):
