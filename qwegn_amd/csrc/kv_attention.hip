@@ -222,8 +222,9 @@ __device__ __forceinline__ float qw_attn_unit(u2_t scales, uint32_t e) {
 // again only where a weight would pass 2^QW_ATTN_ROOM, so that sums and accumulators are hardly ever scaled.  f16 holds up to 2^15.999, 11 bits from 2^-14 on and steps
 // of 2^-24 below: weights from 2^-26 of the largest on have all their bits, n smaller ones are off by n 2^-37 of it.  (Weights of at most one would be lost to the values
 // from 2^-25 on, and stay in the sum.)  Room for a growth of 3.9 digits costs 0 .. 1.5 % over room for 8, 3 digits 2 .. 3 % (a prompt of 4096 rows 195.6, 194.4,
-// 199.3 us).  The wide form's bf16 numbers have fp32's range.
-constexpr float QW_ATTN_UNDER = 12.0f, QW_ATTN_ROOM = 15.9f, QW_ATTN_ROOM_WIDE = 8.0f;
+// 199.3 us).  The wide form's bf16 numbers have fp32's range, and its values may be near
+// the end of it: its weights are at most one, so that no sum leaves the range sooner than in the softmax as it is written.
+constexpr float QW_ATTN_UNDER = 12.0f, QW_ATTN_ROOM = 15.9f, QW_ATTN_ROOM_WIDE = 0.0f;
 
 // A weight's exponent is one multiply-add of the product q.k, which is not rounded in between, but `top` comes from a rounded score: all weights of a column are off by the
 // power of that rounding.  It cancels, but from 2^23 binary digits on it takes weights out of any range.  A range with such a column, from 2^17 on (under it

@@ -116,3 +116,33 @@ def test_scores_far_from_zero(dev, cls, rows, room, t, scale):
             off = np.abs(decode(y[i, h], t).astype(np.float64) - want)
             assert (off <= HALF_STEP[t] * np.abs(want) + 2.0 ** -11 * 1.01 * size + 2.0 ** -25).all(), (i, h, x.max())
             assert abs(l[i, h] - lse) <= 2.0 ** -21 * abs(lse) + 2.0 ** -18, (i, h)
+
+
+@pytest.mark.parametrize("cls,rows,room", ROWS)
+def test_values_near_the_range_of_fp32(dev, cls, rows, room):
+    """Values of 2^125 and scores that grow by less than eight binary digits: a weight is at most one then, and no sum leaves fp32's range that the result does not leave."""
+    n, d = 1500, 64
+    c = cls(dev, 6, d, 1, 4, 16, rows, [n], "bf16", scale=1.0 / 8.0, noise=False)
+    t = np.arange(n)
+    k = np.zeros((n, 1, d))
+    k[:, 0, 0] = np.where(t == 700, 4.0, np.where(t == 1300, 6.0, 0.0))                   # 0, 3.25 and 4.875 nats
+    fill(c, 0, k, np.zeros((n, 1, d)))
+    kc, ks, vc, vs = c.cache.planes()
+    rng = np.random.default_rng(7)
+    v = np.where(np.isin(t, (5, 700, 1300))[:, None], 1.0, 0.0) * np.where(rng.random((1, d)) < 0.5, 1.0, -1.0)
+    fill(c, 0, k, v[:, None] * 4.0)                                                       # elements of 4 under a byte of 127 ..
+    for s in (5, 700, 1300):
+        p, o = c.table[0][s // 16], s % 16
+        assert (vs[p, 0, o // 8, :, o % 8] == 127).all()
+        vs[p, 0, o // 8, :, o % 8] = 250                                                  # .. of 250: 2^125
+    q = np.zeros((c.total, 4, d))
+    q[..., 0] = 6.5
+    c.q = encode(q, "bf16")
+    y, l = c.run(room=room)
+    kk, vv = c.cache.tokens(c.table[0], n)
+    want, lse, size = qwkv.attention(q[: rows[0]], kk, vv, 1.0 / 8.0)
+    got = decode(y[: rows[0]], "bf16").astype(np.float64)
+    assert np.isfinite(want).all() and np.abs(want).min() > 2.0 ** 115
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * size).all()
+    assert (np.abs(l[: rows[0]] - lse) <= 2.0 ** -18).all()
