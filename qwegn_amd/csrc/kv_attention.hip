@@ -54,11 +54,13 @@ __device__ __forceinline__ qw_attn_range qw_attn_tokens(const qw_attn_args& a, c
     r.from = min(part * each, steps), r.to = min(r.from + each, steps);
     return r;
 }
-// Scale bytes of eight tokens from `t` on, of which the ones behind the last are not there: a harmless one in their place.
-__device__ __forceinline__ u2_t qw_attn_tail(u2_t scales, uint32_t t, uint32_t length) {
-    const uint32_t n = length - t, lo = n >= 4u ? ~0u : (1u << (8u * n)) - 1u, hi = n >= 8u ? ~0u : n > 4u ? (1u << (8u * n - 32u)) - 1u : 0u;
-    return u2_t{(scales[0] & lo) | (0x7F7F7F7Fu & ~lo), (scales[1] & hi) | (0x7F7F7F7Fu & ~hi)};
+// Steps begin and end on borders of their own: the tokens of a step that the columns do not see, in front of their window or behind the last, get a harmless scale, so that what
+// is in their places decides nothing, the form neither.  One byte of each of the four tokens from `t` on, set where it is among low .. stop - 1.
+__device__ __forceinline__ uint32_t qw_attn_there(uint32_t t, uint32_t low, uint32_t stop) {
+    const uint32_t behind = t + 4u <= stop ? ~0u : t >= stop ? 0u : (1u << (8u * (stop - t))) - 1u;
+    return behind & (t >= low ? ~0u : t + 4u <= low ? 0u : ~0u << (8u * (low - t)));
 }
+__device__ __forceinline__ uint32_t qw_attn_seen(uint32_t scales, uint32_t there) { return (scales & there) | (0x7F7F7F7Fu & ~there); }
 
 // What a lane carries of a step of 32 tokens, 16 h .. 16 h + 15 in half h.  Keys: rows of an operand of each half, lane (i, g) has elements of its token i; values:
 // lane (i, g) has eight elements of the tokens 4 g .. 4 g + 3 of both halves.  A score of half h, accumulator row 4 g + r, is then token 16 h + 4 g + r: the weights
@@ -88,18 +90,19 @@ __device__ __forceinline__ T qw_attn_codes(const T* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
     else return *p;
 }
-// The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two.  The pages are the same for all lanes: scalar loads and addresses.  ONCE: no other workgroup
+// The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two, of which low .. stop - 1 are seen: a half without one of them is read from the page of the nearest, and
+// masked, so that the table's entries around them are not looked at.  The pages are the same for all lanes: scalar loads and addresses.  ONCE: no other workgroup
 // reads these codes, they pass by the caches.
 template <int D, bool SMALL, bool ONCE>
-__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t t0, uint32_t length,
+__device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t t0, uint32_t low, uint32_t stop,
                                              const qw_attn_place<D>& at, qw_attn_step<D>& s) {
     constexpr uint32_t SETS = qw_attn_step<D>::SETS, WORDS = qw_attn_step<D>::WORDS;
-    const uint32_t page0 = (uint32_t)table[t0 >> a.geo.page_log2];
+    const uint32_t page0 = (uint32_t)table[(SMALL ? max(t0, low) : t0) >> a.geo.page_log2];
     const uint8_t* piece[2];
     uint32_t in[2] = {t0 & ((1u << a.geo.page_log2) - 1u), 0u};
     piece[0] = head + (uint64_t)(page0 < a.page_count ? page0 : 0u) * stride;
     if constexpr (SMALL) {
-        const uint32_t page1 = (uint32_t)table[min(t0 + 16u, length - 1u) >> 4];   // a half behind the last token is read from the last page, and masked
+        const uint32_t page1 = (uint32_t)table[min(t0 + 16u, stop - 1u) >> 4];
         piece[1] = head + (uint64_t)(page1 < a.page_count ? page1 : 0u) * stride;
     } else {
         piece[1] = piece[0];
@@ -120,16 +123,15 @@ __device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_
         }
     }
 }
-// Tokens behind the last one: harmless scales.
 template <int D>
-__device__ __forceinline__ void qw_attn_cut(uint32_t t0, uint32_t length, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
+__device__ __forceinline__ void qw_attn_cut(uint32_t t0, uint32_t low, uint32_t stop, uint32_t i, uint32_t g, qw_attn_step<D>& s) {
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t t = t0 + 16u * h + 4u * g, there = t + 4u <= length ? ~0u : t >= length ? 0u : (1u << (8u * (length - t))) - 1u;
+        const uint32_t key = t0 + 16u * h + i, there = qw_attn_there(t0 + 16u * h + 4u * g, low, stop);
 #pragma unroll
         for (uint32_t c = 0; c < qw_attn_step<D>::SETS; ++c) {
-            if (t0 + 16u * h + i >= length) s.k_scale[h][c] = 127u;
-            s.v_scale[c][h] = (s.v_scale[c][h] & there) | (0x7F7F7F7Fu & ~there);
+            if (key < low || key >= stop) s.k_scale[h][c] = 127u;
+            s.v_scale[c][h] = qw_attn_seen(s.v_scale[c][h], there);
         }
     }
 }
@@ -298,6 +300,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     qw_attn_range t = qw_attn_tokens<32>(a, s, c0, min(c0 + 15u, count - 1u), 0u);
     t.first = max(t.first, begin), t.from = 0u;
     t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
+    const uint32_t stop = s.length;
     // this lane's column
     const uint32_t col = min(c0 + i, count - 1u), row = col / a.shared, member = col - row * a.shared;
     const int32_t pos = s.pos0 + (int32_t)row, low = (int32_t)qw_attn_low(a, pos);
@@ -322,7 +325,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     place.set(a, i, g);
 
     auto one = [&](uint32_t t0, qw_attn_step<D>& now) {
-        if (t0 + 32u > s.length) qw_attn_cut<D>(t0, s.length, i, g, now);
+        if (t0 < t.low_a || t0 + 32u > stop) qw_attn_cut<D>(t0, t.low_a, stop, i, g, now);
         if constexpr (!WIDE) {
 #pragma unroll
             for (uint32_t c = 0; c < SETS; ++c) {
@@ -439,7 +442,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     };
     if (wave < t.to) {
         // wave w has the steps w, w + 4, ..
-        auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL, ONCE>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), s.length, place, f); };
+        auto load = [&](uint32_t step, qw_attn_step<D>& f) { qw_attn_load<D, SMALL, ONCE>(a, pages, stride, table, t.first + 32u * min(step, t.to - 1u), t.low_a, stop, place, f); };
         qw_attn_step<D> f[WIDE ? 1 : 2];
         if constexpr (WIDE) {
             for (uint32_t step = wave; step < t.to; step += 4u) {
@@ -581,7 +584,8 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
     const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
     // A tile lies in one page, the same for all threads (BIG: scalar loads and addresses), or in several small ones.
-    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last_page = (s.length - 1u) >> a.geo.page_log2, last = max(rg.to, 1u) - 1u;   // read only where there are steps
+    const uint32_t stop = s.length, first_page = rg.low_a >> a.geo.page_log2, last_page = (stop - 1u) >> a.geo.page_log2;   // read only where there are steps
+    const uint32_t inside = (1u << a.geo.page_log2) - 1u, last = max(rg.to, 1u) - 1u;
     const uint32_t kin = BIG ? kt : kt & inside, vin = BIG ? vt : vt & inside, kpage = BIG ? 0u : kt >> a.geo.page_log2, vpage = BIG ? 0u : vt >> a.geo.page_log2;
     const uint32_t k_at = kin * (D / 2u) + kw * 4u, ks_at = a.geo.k_scales + kin * (D / 32u) + kw / 4u;
     const uint32_t v_at = a.geo.v_codes + ((vin >> 3) * W + vw) * 32u, vs_at = a.geo.v_scales + ((vin >> 3) * (D / 32u) + vw / 4u) * 8u;
@@ -589,9 +593,12 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     const uint32_t stride = a.kv_heads * a.geo.piece;
     const int32_t* const table = a.table + (uint64_t)seq * a.ld_table;
     auto tile_of = [&](uint32_t step) { return rg.first + min(step, last) * T; };   // first token; behind the last tile the last one's
+    // whether only some of a tile's tokens are seen; whole ones begin at whole .. whole + wholes
+    const uint32_t whole = stop - rg.low_a >= T ? rg.low_a : ~0u, wholes = stop - rg.low_a >= T ? stop - T - rg.low_a : 0u;
+    auto part_of = [&](uint32_t t0) { return t0 - whole > wholes; };
     auto page_at = [&](uint32_t t0, uint32_t more) {
-        const uint32_t p = (t0 >> a.geo.page_log2) + more;   // a part of a tile behind the last token is read from the last page, and masked
-        return (uint32_t)table[BIG ? p : min(p, last_page)];
+        const uint32_t p = (t0 >> a.geo.page_log2) + more;   // a part of a tile in front of the first token that is seen, or behind the last, is read from theirs, and masked
+        return (uint32_t)table[BIG ? p : min(max(p, first_page), last_page)];
     };
     auto base_of = [&](uint32_t page) { return pages + (uint64_t)(page < a.page_count ? page : 0u) * stride; };
     auto fetch_k = [&](uint32_t t0, uint32_t page, qw_attn_fetch<D>& f) {
@@ -610,7 +617,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     };
     auto turn_k = [&](const qw_attn_fetch<D>& f, uint32_t t0, uint32_t slot) {
         uint32_t byte = f.k_scale;
-        if (t0 + T > s.length) byte = t0 + kt >= s.length ? 127u : byte;   // behind the last token: a harmless scale
+        if (part_of(t0)) byte = t0 + kt < rg.low_a || t0 + kt >= stop ? 127u : byte;
         far |= qw_attn_far<DT>(byte);
         const float unit = __uint_as_float(byte << 23);
         const uint32_t t = kt & 31u, at = (t & 16u) | ((t & 4u) << 1) | ((t & 8u) >> 1) | (t & 3u);
@@ -622,7 +629,8 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     };
     auto turn_v = [&](const qw_attn_fetch<D>& f, uint32_t t0, uint32_t slot) {
         u2_t scales = f.v_scale;
-        if (t0 + T > s.length) scales = t0 + vt >= s.length ? u2_t{0x7F7F7F7Fu, 0x7F7F7F7Fu} : qw_attn_tail(scales, t0 + vt, s.length);
+        if (part_of(t0))
+            scales = u2_t{qw_attn_seen(scales[0], qw_attn_there(t0 + vt, rg.low_a, stop)), qw_attn_seen(scales[1], qw_attn_there(t0 + vt + 4u, rg.low_a, stop))};
         far |= qw_attn_far8(scales);
 #pragma unroll
         for (uint32_t i = 0; i < L::VS; ++i) {
