@@ -300,7 +300,7 @@ __device__ __forceinline__ bool qw_attn_stream(const qw_attn_args& a, const qw_a
     qw_attn_range t = qw_attn_tokens<32>(a, s, c0, min(c0 + 15u, count - 1u), 0u);
     t.first = max(t.first, begin), t.from = 0u;
     t.to = t.pos_b < 0 || t.first >= end ? 0u : (min(end, (uint32_t)t.pos_b + 1u) + 31u - min(t.first, (uint32_t)t.pos_b + 1u)) / 32u;
-    const uint32_t stop = s.length;
+    const uint32_t stop = (uint32_t)t.pos_b + 1u;   // behind what they see; read only where there are steps
     // this lane's column
     const uint32_t col = min(c0 + i, count - 1u), row = col / a.shared, member = col - row * a.shared;
     const int32_t pos = s.pos0 + (int32_t)row, low = (int32_t)qw_attn_low(a, pos);
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void qw_attn_tile_kernel(con
     // what this thread turns: token kt, words kw .. of the keys; eight tokens vt .., word vw, pairs vs .. of the values
     const uint32_t kt = tid % T, kw = tid / T * L::KW, vw = tid % W, vt = tid / W % (T / 8u) * 8u, vs = tid / W / (T / 8u) * L::VS;
     // A tile lies in one page, the same for all threads (BIG: scalar loads and addresses), or in several small ones.
-    const uint32_t stop = s.length, first_page = rg.low_a >> a.geo.page_log2, last_page = (stop - 1u) >> a.geo.page_log2;   // read only where there are steps
+    const uint32_t stop = (uint32_t)rg.pos_b + 1u, first_page = rg.low_a >> a.geo.page_log2, last_page = (stop - 1u) >> a.geo.page_log2;   // read only where there are steps
     const uint32_t inside = (1u << a.geo.page_log2) - 1u, last = max(rg.to, 1u) - 1u;
     const uint32_t kin = BIG ? kt : kt & inside, vin = BIG ? vt : vt & inside, kpage = BIG ? 0u : kt >> a.geo.page_log2, vpage = BIG ? 0u : vt >> a.geo.page_log2;
     const uint32_t k_at = kin * (D / 2u) + kw * 4u, ks_at = a.geo.k_scales + kin * (D / 32u) + kw / 4u;

@@ -78,3 +78,22 @@ def test_tokens_in_front_of_a_window_in_its_first_page(dev, cls, d, page, rows, 
         got = c.run(room=1 << 26)
         c.cache.bytes[:] = kept
         assert bits((y, got[0]), (l, got[1])), window
+
+
+@pytest.mark.parametrize("cls,d,page,rows", [(Case, 64, 16, 30), (Case, 128, 64, 30), (Case, 256, 32, 20), (Tiles, 64, 16, 130), (Tiles, 64, 128, 130), (Tiles, 128, 64, 130)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_tokens_behind_a_tiles_last_row(dev, cls, d, page, rows, t):
+    """The last tokens of a prompt broken or out of range: the rows whose tiles end in front of them keep their bits."""
+    c = cls(dev, d + rows, d, 2, 4, page, [rows], [rows], t)
+    y, l = c.run(room=0)
+    kc, ks, vc, vs = c.cache.planes()
+    columns = 16 if cls is Case else 128
+    for tile in range(1, rows * 4 // columns):
+        first = tile * columns // 4                                                       # the tile's first row, and its position
+        kept = c.cache.bytes.copy()
+        for token in range(first, rows):
+            p, o = c.table[0][token // page], token % page
+            ks[p, :, o], vs[p, :, o // 8, :, o % 8] = (230, 255)[token % 2], (255, 99)[token % 2]
+        got = c.run(room=0)
+        c.cache.bytes[:] = kept
+        assert bits((y[:first], got[0][:first]), (l[:first], got[1][:first])), tile
