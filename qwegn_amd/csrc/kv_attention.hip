@@ -860,8 +860,9 @@ constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch 
 // Streaming: powers of two, so that one part of all heads and tiles meets in one XCD's L2 (8 sequences of 8 rows behind 4096 in 1 / 2 / 3 / 4 / 5 / 8 parts 24 / 23 / 24 /
 // 20 / 23 / 24 us).  A workgroup a range: up to 16 parts two workgroups a compute unit, more for one, of at least 128 tokens (a token behind 131077 in 16 / 32 / 48: 47 / 30 /
 // 33; 4 sequences of up to 32768 in 4 / 8 / 16 / 32: 46 / 29 / 26 / 29; 24 of up to 8192 in 1 / 2 / 4 / 8: 44 / 38 / 35 / 36, 64 of them 74 / 77 / 77 / 84; behind 500 in 1 / 4:
-// 7.2 / 8.9).  Several, bound by the vector unit: 256 workgroups, or 1024 of at least 1024 tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 48: 40 / 33 / 32 /
-// 37; 8 rows behind 4096, 24, in 4 / 8 / 16: 13.0 / 11.4 / 12.5).
+// 7.2 / 8.9).  Several, bound by the vector unit: up to 256 workgroups, or 1024 of at least 1024 tokens (16 rows behind 32768, 40 workgroups, in 8 / 16 / 32 / 48: 40 / 33 / 32 /
+// 37; 8 rows behind 4096, 24, in 4 / 8 / 16: 13.0 / 11.4 / 12.5; up to 342 workgroups instead took 10 % longer over 68 shapes that they change: 16 rows behind 1500 in 4 /
+// 8: 11.1 / 12.4, 64 in 1 / 2: 12.2 / 15.3, 20 sequences of 8 rows and heads of 256 in a window of 1000 in 1 / 2: 18.1 / 23.0).
 // Tiles: as many as run at once, else two rounds of them (heads of 64: three), of at least 1536 tokens (heads of 128, two a unit: 160 tiles in 2 / 3 / 4 parts 276 /
 // 207 / 246, two chunks of 512 rows, 320, in 1 / 3 / 4: 242 / 199 / 206, eight of up to 256, 640, in 1 / 2: 142 / 152; heads of 64, three a unit: 192 in 3 / 4 / 6: 190 /
 // 154 / 186; six ragged chunks, 680, in 1 / 2 / 3: 178 / 161 / 152).
@@ -898,7 +899,7 @@ static qw_attn_plan qw_attn_choose(const qwhip_kv_cache* c, const qwhip_kv_batch
                 return two;
             };
             if (p.tiles == 1u) parts = up(512u, all) <= 16u ? up(512u, all) : std::max<uint64_t>(16u, up(256u, all));
-            else parts = down(342u, all);
+            else parts = down(256u, all);
             parts = std::min(parts, down(longest, 128u));
             if (p.tiles > 1u) parts = std::max(parts, std::min(up(1024u, all), down(longest, 1024u)));
         }
