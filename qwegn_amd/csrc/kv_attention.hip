@@ -15,7 +15,7 @@ struct qw_attn_args {
     float* part;           // [parts][rows][q_heads][D] sums, then [parts][rows][q_heads][2] what the weights' exponents are less (`top`) and the sum of weights
     qw_kv_geometry geo;
     uint32_t page_count, kv_heads, ld_table, max_rows, max_length, rows, q_heads, shared, ld_q, ld_out, window, parts, tiles;
-    float scale2;          // scale * log2(e)
+    float scale2, digit, digit_rest;   // scale * log2(e) as fp32 rounds it; what a digit of a score is then, scale / scale2, in two parts
 };
 
 // A sequence's rows and tokens, cut to what the host allows; the position of its first row.
@@ -237,11 +237,14 @@ __device__ __forceinline__ uint32_t qw_attn_far_score(float top) { return fabsf(
 
 // What a row's sums are multiplied by, and the logarithm of its sum.  Maxima are of scaled scores: one under fp32's range is -inf and none at all, and a row
 // without a score over -inf has neither; one over the range is an infinity under which nothing has a finite weight: NaN.  The sum's exponent goes to the maximum
-// first, so that the logarithm of what is left has all of its bits.
+// first, so that the logarithm of what is left has all of its bits, and the digits become a logarithm by what the scale's own rounding made of them: one rounding of fp32
+// in all, and 2^-20 for the weights' exponents.
 __device__ __forceinline__ float qw_attn_inverse(float best, float total) { return best == -__builtin_inff() && total == 0.0f ? 0.0f : 1.0f / total; }
-__device__ __forceinline__ float qw_attn_log(float best, float total) {
+__device__ __forceinline__ float qw_attn_log(const qw_attn_args& a, float best, float total) {
     if (best == -__builtin_inff() && total == 0.0f) return -__builtin_inff();
-    return 0.6931471805599453f * ((best + (float)__builtin_amdgcn_frexp_expf(total)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(total)));
+    const float exponent = (float)__builtin_amdgcn_frexp_expf(total), s = best + exponent, b = s - best, rest = (best - (s - b)) + (exponent - b);   // s + rest: the sum
+    const float less = (rest + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(total))) * a.digit;
+    return __builtin_fmaf(s, a.digit, __builtin_fmaf(s, a.digit_rest, less));
 }
 
 // E elements from `at` on of a row and head: into the output where the range is the whole, else with the range's maximum and sum into the workspace.
@@ -261,7 +264,7 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
     for (uint32_t e = 0; e < E; ++e) o[e] *= inv;
 #pragma unroll
     for (uint32_t e = 0; e < E; e += E < 8u ? E : 8u) qw_attn_store<DT, (E < 8u ? E : 8u)>(y + e, o + e);
-    if (a.lse && first) a.lse[item] = qw_attn_log(best, total);
+    if (a.lse && first) a.lse[item] = qw_attn_log(a, best, total);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -846,7 +849,7 @@ __global__ __launch_bounds__(256) void qw_attn_join_kernel(const qw_attn_args a)
     const float inv = qw_attn_inverse(best, total);
     float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     qw_attn_store<DT, 4>(a.out + (uint64_t)(s.row0 + row) * a.ld_out + (at - row * a.q_heads) * D + lane * 4u, y);
-    if (a.lse && tid % LANES == 0u) a.lse[item] = qw_attn_log(best, total);
+    if (a.lse && tid % LANES == 0u) a.lse[item] = qw_attn_log(a, best, total);
 }
 
 constexpr uint32_t QW_ATTN_MOST_TILES = 1u << 22;   // of 256 threads, a launch holds under 2^32
@@ -983,6 +986,7 @@ extern "C" qwhip_status qwhip_kv_attention_mxfp4(qwhip_stream_t s, const qwhip_k
     a.rows = rows, a.q_heads = q_heads, a.shared = shared, a.ld_q = ld_q, a.ld_out = ld_out, a.window = window > 0x7FFFFFFFu ? 0u : window;
     a.tiles = (uint32_t)plan.tiles;
     a.scale2 = scale * 1.4426950408889634f;
+    a.digit = (float)((double)scale / a.scale2), a.digit_rest = (float)((double)scale / a.scale2 - a.digit);
     a.parts = 1;
     if (workspace) {
         a.parts = plan.parts;

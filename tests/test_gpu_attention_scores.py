@@ -146,3 +146,28 @@ def test_values_near_the_range_of_fp32(dev, cls, rows, room):
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * size).all()
     assert (np.abs(l[: rows[0]] - lse) <= 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("cls,rows,room", ROWS)
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [128.0 ** -0.5, 0.3, 7.1, 1e-6])
+def test_the_logarithm_has_the_precision_of_fp32(dev, cls, rows, room, t, scale):
+    """One token decides (the others lie 30 nats or more below, which fp32's one does not notice) or all do, with a product that is exact in fp32: the logarithm is off by a rounding of a
+    score, one of its own (2^-24 each) and 2^-20 for the exponents of the weights."""
+    n, d = 1700, 64
+    c = cls(dev, 8, d, 1, 4, 32, rows, [n], t, scale=scale, noise=False)
+    rng = np.random.default_rng(9)
+    k = np.zeros((n, 1, d))
+    k[0] = rng.choice([1.0, 1.5, 2.0, 3.0, 4.0], d)                                       # the first token is seen by all rows
+    fill(c, 0, k, rng.standard_normal((n, 1, d)))
+    q = rng.integers(1, 60, (c.total, 4, d)).astype(np.float64)
+    q[:, 3] = 0.0
+    c.q = encode(q, t)
+    y, l = c.run(room=room)
+    kk, _ = c.cache.tokens(c.table[0], n)
+    for i in range(rows[0]):
+        seen = n - rows[0] + i + 1
+        for h in range(4):
+            x = float(q[i, h] @ kk[0, 0]) * float(np.float32(scale))
+            want = np.logaddexp(x, np.log(seen - 1.0))
+            assert abs(l[i, h] - want) <= 2.0 ** -23 * abs(want) + 2.0 ** -20, (i, h, l[i, h], want)
