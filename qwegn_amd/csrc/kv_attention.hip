@@ -91,8 +91,9 @@ __device__ __forceinline__ T qw_attn_codes(const T* p) {
     else return *p;
 }
 // The 32 tokens from t0 on, of one page or (SMALL: pages of 16) two, of which low .. stop - 1 are seen: a half without one of them is read from the page of the nearest, and
-// masked, so that the table's entries around them are not looked at.  The pages are the same for all lanes: scalar loads and addresses.  ONCE: no other workgroup
-// reads these codes, they pass by the caches.
+// masked, so that the table's entries around them are not looked at.  The pages are the same for all lanes: scalar loads and addresses.  ONCE: of a sequence one
+// workgroup reads these codes, they are marked as read once (64 tokens behind 8192 each 99 us, 105 unmarked; sequences that share pages lose nothing by it: all 8192
+// tokens shared 68 us either way).
 template <int D, bool SMALL, bool ONCE>
 __device__ __forceinline__ void qw_attn_load(const qw_attn_args& a, const uint8_t* head, uint32_t stride, const int32_t* table, uint32_t t0, uint32_t low, uint32_t stop,
                                              const qw_attn_place<D>& at, qw_attn_step<D>& s) {
@@ -270,12 +271,12 @@ __device__ __forceinline__ void qw_attn_write(const qw_attn_args& a, uint32_t pa
 // ------------------------------------------------------------------------------------------------
 // Streaming: four waves share 16 columns (query rows of a group of heads) and a range of tokens, a step of 32 tokens of its own each, the next step's codes on their
 // way; all stays in registers.  S^T = K q^T by two operands of 16 tokens; the running maximum of a column over the lanes of the wave; O^T += V^T P^T.  Elements become
-// f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range or a block is broken, which the waves notice at the end of their
-// range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a broken
+// f16 (keys of bf16 queries: bf16) on the way into the matrix unit.  Where a scale leaves f16's range, a block is broken or a score is far from zero, which the waves notice at the end of
+// their range, the range is done once more in the wide form: keys and values in bf16, which holds them all, f16 queries and the weights as two bf16 numbers each, a broken
 // block of values for the rows alone that see its token.
 // One workgroup a range is bound by the bytes: a token of 64 sequences of up to 8192, 40 heads of 128 over 8: 73 us = 5.6 TB/s of codes and scales (a read of 4 GiB
 // 6.15); behind 131077: 30 us (26 = 5.5 TB/s and the join); behind 4096: 8.7 us, latency of two launches.  Several, which read the same tokens from the L2, by the
-// vector unit (201 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17 us.
+// vector unit (200 instructions a wave and step, 96 of them turn elements): 8 rows of 16 windows of 1000 tokens, heads of 256: 17.2 us.
 // Steps on the 64: one wave's registers for both forms 117 us; 128 registers 100; four scale bytes at a time 93; pages by scalar loads, the tail's care in the last step
 // alone, two register sets in turn 85; loads of whole lines, codes as streamed loads 78; three workgroups a unit, not four: 168 registers, so that the
 // loads of a step stay ahead of it 73 (three steps ahead 75, four 77).  The four waves' sums meet in LDS at the end.
@@ -520,10 +521,10 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void qw_attn_
 //   values   operand of 32 elements x 16 tokens, lane (r, h) tokens 8 h .. of element 8 (r % W) + j, W = D / 8 words, r / W picking j in its tile
 // A step: the weights of its tile out of its scores, the next tile turned into LDS, a meeting; its values under its weights and the next tile's scores, 32 matrix
 // instructions in a row whose operands come from LDS eight ahead.  One meeting does: what a wave that is ahead turns goes into the half of LDS that all have left
-// behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: 292 vector instructions a wave and step against 32 matrix ones
-// of 32 cycles, which keep that unit busy for 40 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at its
-// full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 192 .. 197 us by card = 895 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six
-// ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 147 .. 154 us = 510
+// behind them at the meeting before.  Bound by the vector unit beside the matrix unit (heads of 128: 297 vector instructions a wave and step against 32 matrix ones
+// of 32 cycles, which keep that unit busy for 39 % of the cycles; the two workgroups of a compute unit overlap little, and four waves that multiply read LDS at its
+// full rate): 4096 rows of a prompt, 40 heads of 128, bf16: 195 .. 201 us by card = 880 TFLOP/s (the library's product of 8192 x 8192 bf16 matrices: 1230); six
+// ragged chunks of up to 700 rows behind up to 6001 tokens, 24 heads of 64, whose scores cost as much for half the products, in three parts: 157 .. 165 us = 480
 // TFLOP/s.  Steps on the prompt: 16 columns a wave in the streaming kernel 510 us; tiles through LDS 253; scores a tile ahead 215; operands eight reads ahead 208, a
 // wave's priority around them 204; scale bytes four at a time 201; pages and addresses on the scalar unit, one meeting a step 196.  Eight waves a workgroup turn a
 // tile for twice the columns, but meet more of each other (245); two groups of waves half a step apart leave a SIMD's vector unit to one wave at a time (252);
